@@ -56,6 +56,10 @@ _I64 = C.c_int64
 _PP = C.POINTER(C.c_void_p)
 _PI32 = C.POINTER(C.c_int32)
 
+DTYPE_BF16 = 0
+DTYPE_F16 = 1
+DTYPE_F32 = 2
+
 _SIGS = {
     "gsec_last_error": (C.c_char_p, []),
     "gsec_version": (C.c_char_p, []),
@@ -73,6 +77,13 @@ _SIGS = {
                                           _P]),
     "gsec_slots_scatter_pools": (C.c_int, [_PP, _I32, _I64, _I64, _I32, _I64, _P, _I32, _I64, _I64, _P, _P, _I64,
                                            _P]),
+    "gsec_slots_plan": (C.c_int, [_P, _P, _I32, _P, _I64, _I32, _P, _I64, _P, _I32, _I32, _P, _P, _I64, _P, _P, _P,
+                                  _P]),
+    "gsec_qk_norm_rope_store": (C.c_int, [_P, _I64, _I64, _I32, _I32, _I32, _I32, _P, _P, _I64, _I64, _I64, _P, _I32,
+                                          _P, _I32, _P, _P, _I32, _I64, _P, _P, C.c_float, _I32, _P]),
+    "gsec_prefix_attention": (C.c_int, [_P, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _P, _I64, _I64, _I64, _P, _P,
+                                        _I32, _P, _I64, _I32, _I32, _P, _I64, C.c_float, _P, _P, _P, _I64, _P]),
+    "gsec_prefix_attention_workspace": (C.c_int, [_I64, _I32, _I64, _I32, _I32, _I32, _I32, C.POINTER(_I64)]),
     "gsec_xor_encode": (C.c_int, [_P, _P, _I32, _I64, _I64, _P]),
     "gsec_xor_reconstruct": (C.c_int, [_P, _P, _I64, _I64, _I32, _PI32, _I32, _P]),
     "gsec_rdpref_pack_row": (C.c_int, [_P, _P, _I64, _P, _I64, _I32, _P]),

@@ -11,7 +11,9 @@
 #include <string>
 #include <vector>
 
+#include "attention.cuh"
 #include "common.cuh"
+#include "kvpool.cuh"
 #include "layout.cuh"
 #include "linear.cuh"
 #include "rdp.cuh"
@@ -250,9 +252,12 @@ int gsec_device_status(uint32_t* status, int32_t clear) {
   const unsigned v2 = linear_device_status(clear != 0);
   const unsigned v3 = layout_device_status(clear != 0);
   const unsigned v4 = gather_device_status(clear != 0);
-  const unsigned v = (v1 == 0xffffffffu || v2 == 0xffffffffu || v3 == 0xffffffffu || v4 == 0xffffffffu)
+  const unsigned v5 = kvpool_device_status(clear != 0);
+  const unsigned v6 = attention_device_status(clear != 0);
+  const unsigned v = (v1 == 0xffffffffu || v2 == 0xffffffffu || v3 == 0xffffffffu || v4 == 0xffffffffu ||
+                      v5 == 0xffffffffu || v6 == 0xffffffffu)
                          ? 0xffffffffu
-                         : (v1 | (v2 << 8) | (v3 << 16) | (v4 << 24));
+                         : (v1 | (v2 << 8) | ((v3 | v5 | ((v6 & 1u) << 3)) << 16) | ((v4 | (v6 & 2u)) << 24));
   if (v == 0xffffffffu) {
     set_error("cannot read the device status word");
     return GSEC_ECUDA;
@@ -552,6 +557,180 @@ int gsec_slots_scatter_pools(void* const* pools, int32_t npools, int64_t pitch, 
   if (rc) return rc;
   return slots_move(false, pools, npools, pitch, plane, nplanes, row_bytes, slots, slot_bytes, n, pool_rows,
                     const_cast<void*>(src_lo), const_cast<void*>(src_hi), split, as_stream(stream));
+}
+
+// --------------------------------------------------- serving a paged pool ---
+namespace {
+int dtype_bytes(int32_t dtype) { return dtype == GSEC_F32 ? 4 : 2; }
+
+// Head layout shared by the store and the attention: types, head counts, and
+// vectors of 16 bytes throughout.
+int heads_ok(int32_t dtype, int32_t hq, int32_t hk, int32_t dim, const void* pool, int64_t pitch, int64_t plane,
+             int64_t pool_rows) {
+  GSEC_REQUIRE(dtype == GSEC_BF16 || dtype == GSEC_F16 || dtype == GSEC_F32, "dtype=%d must be bf16, fp16 or fp32",
+               dtype);
+  GSEC_REQUIRE(hk >= 1 && hq >= 1 && hq <= 4096 && hq % hk == 0, "hq=%d must be a multiple of hk=%d, at most 4096", hq,
+               hk);
+  GSEC_REQUIRE(dim >= 1 && dim <= 256 && dim * dtype_bytes(dtype) % 16 == 0,
+               "dim=%d must be whole 16-byte vectors, at most 256 values", dim);
+  GSEC_REQUIRE(pool != nullptr && aligned16(pool) && (pitch & 15) == 0 && (plane & 15) == 0,
+               "pool, pitch and plane offset must be 16-byte aligned");
+  // K and V rows side by side in a slot's record, or two planes of all slots one after the other
+  const int64_t row = (int64_t)hk * dim * dtype_bytes(dtype);
+  GSEC_REQUIRE(pool_rows >= 0 && pitch >= row && plane >= row && pitch < (1ll << 40) && pool_rows < (1ll << 40),
+               "slot record: pitch and plane offset must be at least a row of %lld bytes", (long long)row);
+  GSEC_REQUIRE(plane <= pitch - row || pool_rows == 0 || plane / pitch >= pool_rows - (plane % pitch >= row ? 1 : 0),
+               "slot record: K and V rows overlap");
+  return GSEC_OK;
+}
+}  // namespace
+
+int gsec_slots_plan(const int32_t* lens, const int32_t* new_lens, int32_t batch, int32_t* table, int64_t table_pitch,
+                    int32_t width, const int32_t* free_pages, int64_t nfree, const int32_t* cursor, int32_t page,
+                    int32_t base, int64_t* slots, int32_t* positions, int64_t capacity, int32_t* cu,
+                    int32_t* lens_out, int32_t* cursor_out, gsec_stream_t stream) {
+  GSEC_REQUIRE(batch >= 1 && batch <= kPlanMaxBatch, "batch=%d must be in [1, %d]", batch, kPlanMaxBatch);
+  GSEC_REQUIRE(lens && new_lens && table && cursor && cu && lens_out && cursor_out, "null pointer");
+  GSEC_REQUIRE((nfree == 0 || free_pages) && (capacity == 0 || (slots && positions)), "null pointer");
+  GSEC_REQUIRE(page >= 1 && width >= 1 && table_pitch >= width && nfree >= 0, "bad page/width/table_pitch/nfree");
+  GSEC_REQUIRE(capacity >= 0 && capacity < (1ll << 31), "capacity must be in [0, 2^31)");
+  GSEC_REQUIRE(aligned16(slots) && aligned16(positions), "slots and positions must be 16-byte aligned");
+  GSEC_REQUIRE(lens_out != lens && lens_out != new_lens && cursor_out != cursor,
+               "lens_out and cursor_out must not be the inputs");
+  SlotPlanArgs a{};
+  a.lens = lens;
+  a.fresh = new_lens;
+  a.batch = batch;
+  a.table = table;
+  a.table_pitch = table_pitch;
+  a.width = width;
+  a.free_pages = free_pages;
+  a.nfree = nfree;
+  a.cursor = cursor;
+  a.page = page;
+  a.page_div = FastDiv((uint32_t)page);
+  a.base = base;
+  a.slots = slots;
+  a.positions = positions;
+  a.capacity = capacity;
+  a.cu = cu;
+  a.lens_out = lens_out;
+  a.cursor_out = cursor_out;
+  return slots_plan(a, as_stream(stream));
+}
+
+int gsec_qk_norm_rope_store(const void* qkv, int64_t qkv_pitch, int64_t tokens, int32_t dtype, int32_t hq, int32_t hk,
+                            int32_t dim, void* q_out, void* pool, int64_t pitch, int64_t plane, int64_t pool_rows,
+                            const void* slots, int32_t slot_bytes, const void* positions, int32_t position_bytes,
+                            const float* cos, const float* sin, int32_t rot, int64_t max_pos, const void* q_weight,
+                            const void* k_weight, float eps, int32_t interleaved, gsec_stream_t stream) {
+  const int rc = heads_ok(dtype, hq, hk, dim, pool, pitch, plane, pool_rows);
+  if (rc) return rc;
+  const int es = dtype_bytes(dtype);
+  GSEC_REQUIRE(tokens >= 0 && tokens < (1ll << 31), "tokens must be in [0, 2^31)");
+  GSEC_REQUIRE(tokens == 0 || (qkv && q_out && slots && positions), "null pointer");
+  GSEC_REQUIRE(dim * es <= 512, "dim=%d: a head is at most 512 bytes", dim);
+  GSEC_REQUIRE(slot_bytes == 4 || slot_bytes == 8, "slot_bytes=%d must be 4 or 8", slot_bytes);
+  GSEC_REQUIRE(position_bytes == 4 || position_bytes == 8, "position_bytes=%d must be 4 or 8", position_bytes);
+  GSEC_REQUIRE(rot >= 0 && rot <= dim && (rot * es) % 32 == 0, "rot=%d must be two halves of 16-byte vectors within dim",
+               rot);
+  GSEC_REQUIRE(max_pos >= 0 && (rot == 0 || (cos && sin)), "null pointer (cos, sin)");
+  GSEC_REQUIRE(aligned16(qkv) && (qkv_pitch & 15) == 0 && aligned16(q_out) && aligned16(q_weight) &&
+                   aligned16(k_weight),
+               "qkv, its pitch, q_out and the weights must be 16-byte aligned");
+  GSEC_REQUIRE(qkv_pitch >= (int64_t)(hq + 2 * hk) * dim * es, "qkv rows overlap");
+  QkStoreArgs a{};
+  a.qkv = static_cast<const char*>(qkv);
+  a.qkv_pitch = qkv_pitch;
+  a.tokens = tokens;
+  a.hq = hq;
+  a.hk = hk;
+  a.dim = dim;
+  a.q_out = static_cast<char*>(q_out);
+  a.pool = static_cast<char*>(pool);
+  a.pitch = pitch;
+  a.plane = plane;
+  a.pool_rows = pool_rows;
+  a.slots = slots;
+  a.positions = positions;
+  a.cos = cos;
+  a.sin = sin;
+  a.rot = rot;
+  a.max_pos = max_pos;
+  a.q_weight = q_weight;
+  a.k_weight = k_weight;
+  a.eps = eps;
+  a.interleaved = interleaved != 0;
+  return qk_norm_rope_store(a, dtype, slot_bytes, position_bytes, as_stream(stream));
+}
+
+int gsec_prefix_attention_workspace(int64_t tokens, int32_t batch, int64_t prefix_len, int32_t dtype, int32_t hq,
+                                    int32_t hk, int32_t dim, int64_t* bytes) {
+  GSEC_REQUIRE(bytes != nullptr && tokens >= 0 && batch >= 0 && prefix_len >= 0 && hk >= 1 && hq >= 1 && hq % hk == 0 &&
+                   dim >= 1,
+               "bad sizes");
+  AttnArgs a{};
+  a.tokens = tokens;
+  a.batch = batch;
+  a.prefix_len = (int32_t)prefix_len;
+  a.hq = hq;
+  a.hk = hk;
+  a.group = hq / hk;
+  a.dim = dim;
+  *bytes = attention_workspace(a, dtype);
+  return GSEC_OK;
+}
+
+int gsec_prefix_attention(const void* q, int64_t q_pitch, int64_t q_head, int64_t tokens, int32_t dtype, int32_t hq,
+                          int32_t hk, int32_t dim, const void* pool, int64_t pitch, int64_t plane, int64_t pool_rows,
+                          const int32_t* cu, const int32_t* lens, int32_t batch, const int32_t* table,
+                          int64_t table_pitch, int32_t width, int32_t page, const int32_t* prefix, int64_t prefix_len,
+                          float scale, void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                          gsec_stream_t stream) {
+  const int rc = heads_ok(dtype, hq, hk, dim, pool, pitch, plane, pool_rows);
+  if (rc) return rc;
+  GSEC_REQUIRE(tokens >= 0 && tokens * hq < (1ll << 31), "tokens * hq must be below 2^31");
+  if (tokens == 0) return GSEC_OK;
+  GSEC_REQUIRE(batch >= 1 && batch <= kPlanMaxBatch, "batch=%d must be in [1, %d]", batch, kPlanMaxBatch);
+  GSEC_REQUIRE(q && out && cu && lens && (prefix_len == 0 || prefix), "null pointer");
+  GSEC_REQUIRE(width >= 0 && (width == 0 || table) && table_pitch >= width && page >= 1, "bad table, width or page");
+  GSEC_REQUIRE(prefix_len >= 0 && prefix_len + (int64_t)width * page < (1ll << 30),
+               "prefix and table hold at most 2^30 keys");
+  GSEC_REQUIRE(aligned16(q) && (q_pitch & 15) == 0 && (q_head & 15) == 0 && aligned16(out),
+               "q, its strides and out must be 16-byte aligned");
+  GSEC_REQUIRE(scale == scale && scale < 3e38f && scale > -3e38f, "scale must be finite");
+  AttnArgs a{};
+  a.q = static_cast<const char*>(q);
+  a.q_pitch = q_pitch;
+  a.q_head = q_head;
+  a.tokens = tokens;
+  a.hq = hq;
+  a.hk = hk;
+  a.group = hq / hk;
+  a.dim = dim;
+  a.pool = static_cast<const char*>(pool);
+  a.pitch = pitch;
+  a.plane = plane;
+  a.pool_rows = pool_rows;
+  a.cu = cu;
+  a.lens = lens;
+  a.batch = batch;
+  a.table = table;
+  a.table_pitch = table_pitch;
+  a.width = width;
+  a.page = page;
+  a.page_div = FastDiv((uint32_t)page);
+  a.group_div = FastDiv((uint32_t)a.group);
+  a.prefix = prefix;
+  a.prefix_len = (int32_t)prefix_len;
+  a.scale = scale;
+  a.out = static_cast<char*>(out);
+  a.lse = lse;
+  a.workspace = static_cast<char*>(workspace);
+  const int64_t need = attention_workspace(a, dtype);
+  GSEC_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need),
+               "workspace: needs %lld bytes, 16-byte aligned", (long long)need);
+  return attention(a, dtype, as_stream(stream));
 }
 
 int gsec_copy_gather(const void* const* src, const int64_t* bytes, int32_t n, void* dst, gsec_stream_t stream) {

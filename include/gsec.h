@@ -70,7 +70,8 @@ GSEC_API const char* gsec_version(void);
  * wait; one that gives up sets a bit here and returns early, so a non-zero
  * status means some call since the last clear produced incomplete output.
  * clear != 0 resets it. No counterpart in the reference (its kernels have no
- * waits). */
+ * waits). Bits 17 to 19 and 25: see gsec_slots_plan, gsec_qk_norm_rope_store and
+ * gsec_prefix_attention. */
 GSEC_API int gsec_device_status(uint32_t* status, int32_t clear);
 
 /* ------------------------------------------------------------------------- */
@@ -153,6 +154,81 @@ GSEC_API int gsec_slots_gather(const void* pool, int64_t pitch, int64_t plane, i
 GSEC_API int gsec_slots_scatter(void* pool, int64_t pitch, int64_t plane, int32_t nplanes,
                        int64_t row_bytes, const void* slots, int32_t slot_bytes, int64_t n,
                        int64_t pool_rows, const void* src, gsec_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
+/* Serving a paged KV pool: slot plan, store of new tokens, attention          */
+/* (no counterpart in the reference, whose server brings its own)              */
+/* ------------------------------------------------------------------------- */
+
+/* Element types of the serving entries. */
+enum { GSEC_BF16 = 0, GSEC_F16 = 1, GSEC_F32 = 2 };
+
+/* Plan the slots of a batch's new tokens. Request i (batch <= 16384) holds
+ * lens[i] tokens on the first ceil(lens[i] / page) pages of its row of `table`
+ * ([batch, width] int32, table_pitch elements apart) and gets new_lens[i] more.
+ * The pages that needs are taken in request order from free_pages[cursor[0]..)
+ * and appended to the row; slot = page id * page + offset. Outputs:
+ * cu[0..batch] = exclusive sums of new_lens; lens_out = lens + new_lens;
+ * cursor_out[0] = cursor[0] + pages taken; and for token t of the batch (request
+ * by request) slots[t] and positions[t] = base + its index in the request. Rows
+ * from cu[batch] to capacity get slot -1 and position 0. All arrays are on the
+ * device; slots and positions are 16-byte aligned; lens_out and cursor_out are
+ * not lens and cursor. Missing free pages, a row past `width`, tokens past
+ * `capacity` or a negative length set bit 17 of gsec_device_status; a token
+ * without a page gets slot -1. */
+GSEC_API int gsec_slots_plan(const int32_t* lens, const int32_t* new_lens, int32_t batch, int32_t* table,
+                    int64_t table_pitch, int32_t width, const int32_t* free_pages, int64_t nfree,
+                    const int32_t* cursor, int32_t page, int32_t base, int64_t* slots,
+                    int32_t* positions, int64_t capacity, int32_t* cu, int32_t* lens_out,
+                    int32_t* cursor_out, gsec_stream_t stream);
+
+/* Norm, rotate and store a batch's new queries and keys in one pass. Row t of
+ * qkv (qkv_pitch bytes apart) is hq query, hk key and hk value heads of `dim`
+ * values of `dtype`. Query and key heads are divided by their root mean square
+ * and multiplied by q_weight / k_weight ([dim], null: no norm); then the first
+ * `rot` values turn by row positions[t] of cos and sin ([max_pos, rot / 2]
+ * fp32): pairs (i, i + rot/2), or neighbours when interleaved. Queries go to
+ * q_out ([tokens, hq, dim]); keys and values to slot record slots[t] of the pool
+ * (pitch bytes apart, V at byte `plane`: beside K in the record, or past all K
+ * rows; a negative slot stores nothing; no slot twice). Arithmetic
+ * is in 32 bits, rounded once. slot_bytes / position_bytes: 4 or 8. dim: a
+ * multiple of 16 bytes, at most 512 bytes; rot: two halves of whole 16-byte
+ * vectors. A slot >= pool_rows stores nothing and sets bit 16 of
+ * gsec_device_status, a position outside the tables leaves the row unrotated
+ * and sets bit 18. */
+GSEC_API int gsec_qk_norm_rope_store(const void* qkv, int64_t qkv_pitch, int64_t tokens, int32_t dtype, int32_t hq,
+                            int32_t hk, int32_t dim, void* q_out, void* pool, int64_t pitch,
+                            int64_t plane, int64_t pool_rows, const void* slots,
+                            int32_t slot_bytes, const void* positions, int32_t position_bytes,
+                            const float* cos, const float* sin, int32_t rot, int64_t max_pos,
+                            const void* q_weight, const void* k_weight, float eps,
+                            int32_t interleaved, gsec_stream_t stream);
+
+/* Attention of a ragged batch over a paged pool with a shared prefix. Query
+ * tokens cu[i]..cu[i+1) of request i (n of them) attend to the prefix_len keys
+ * on the pages `prefix` and to the request's own keys (lens[i], on its row of
+ * `table`): token j sees own keys 0 .. lens[i] - n + j. hq / hk query heads read
+ * each KV head. out ([tokens, hq, dim]) and lse ([tokens, hq], natural log, may
+ * be null); a row that sees no key is 0 and -inf, rows from cu[batch] on are not
+ * written. q: byte strides q_pitch (token) and q_head (head). dim: whole 16-byte
+ * vectors, at most 256 values. Own and prefix keys and values that a row does not
+ * see must be finite where another row of the same request sees them; slots
+ * outside all lengths may hold anything. workspace: 16-byte aligned, of
+ * gsec_prefix_attention_workspace bytes (0 with the same tokens, heads and dim
+ * means none is needed), not shared by calls that may overlap. A page outside the
+ * pool reads as zeros, a length past the table or a batch past `tokens` is cut;
+ * both set bit 19 of gsec_device_status. A bounded wait that gives up sets bit
+ * 25. */
+GSEC_API int gsec_prefix_attention(const void* q, int64_t q_pitch, int64_t q_head, int64_t tokens, int32_t dtype,
+                          int32_t hq, int32_t hk, int32_t dim, const void* pool, int64_t pitch,
+                          int64_t plane, int64_t pool_rows, const int32_t* cu,
+                          const int32_t* lens, int32_t batch, const int32_t* table,
+                          int64_t table_pitch, int32_t width, int32_t page,
+                          const int32_t* prefix, int64_t prefix_len, float scale, void* out,
+                          float* lse, void* workspace, int64_t workspace_bytes,
+                          gsec_stream_t stream);
+GSEC_API int gsec_prefix_attention_workspace(int64_t tokens, int32_t batch, int64_t prefix_len, int32_t dtype,
+                                    int32_t hq, int32_t hk, int32_t dim, int64_t* bytes);
 
 /* One-kernel gather: dst = src[0][0..bytes[0]) ++ ... ++ src[n-1][0..bytes[n-1])
  * (n <= 32; every source, size and dst 16-byte aligned/multiple of 16). Sources
