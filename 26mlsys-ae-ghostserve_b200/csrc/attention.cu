@@ -132,9 +132,9 @@ __global__ void __launch_bounds__(kRowThreads) attend_row_kernel(const AttnArgs 
     for (int g = 0; g < ngrp; ++g)
       if (sm[g * (a.dim + 2) + a.dim] > -INFINITY)
         x += sm[g * (a.dim + 2) + d] * exp2f(sm[g * (a.dim + 2) + a.dim] - top);
-    reinterpret_cast<T*>(a.out)[(t * a.hq + h) * a.dim + d] = (T)(sum > 0.f ? x / sum : 0.f);
+    reinterpret_cast<T*>(a.out)[(t * a.hq + h) * a.dim + d] = (T)(sum == 0.f ? 0.f : x / sum);
   }
-  if (threadIdx.x == 0 && a.lse) a.lse[t * a.hq + h] = sum > 0.f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+  if (threadIdx.x == 0 && a.lse) a.lse[t * a.hq + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
 template <typename T, int NC>
