@@ -14,6 +14,7 @@ template <typename T>
 struct Vec16;
 template <>
 struct Vec16<__nv_bfloat16> {
+  static constexpr bool bf16 = true;
   static constexpr int N = 8;
   static __device__ __forceinline__ void unpack(const uint4& v, float* f) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -33,6 +34,7 @@ struct Vec16<__nv_bfloat16> {
 };
 template <>
 struct Vec16<__half> {
+  static constexpr bool bf16 = false;
   static constexpr int N = 8;
   static __device__ __forceinline__ void unpack(const uint4& v, float* f) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
