@@ -692,6 +692,7 @@ int gsec_prefix_attention(const void* q, int64_t q_pitch, int64_t q_head, int64_
   GSEC_REQUIRE(tokens >= 0 && tokens * hq < (1ll << 31), "tokens * hq must be below 2^31");
   if (tokens == 0) return GSEC_OK;
   GSEC_REQUIRE(batch >= 1 && batch <= kPlanMaxBatch, "batch=%d must be in [1, %d]", batch, kPlanMaxBatch);
+  GSEC_REQUIRE(pool_rows >= 1 && pool_rows < (1ll << 31), "pool_rows must be in [1, 2^31)");
   GSEC_REQUIRE(q && out && cu && lens && (prefix_len == 0 || prefix), "null pointer");
   GSEC_REQUIRE(width >= 0 && (width == 0 || table) && table_pitch >= width && page >= 1, "bad table, width or page");
   GSEC_REQUIRE(prefix_len >= 0 && prefix_len + (int64_t)width * page < (1ll << 30),

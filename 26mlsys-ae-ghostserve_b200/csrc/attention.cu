@@ -186,6 +186,7 @@ constexpr int kLaunchRegs = 168, kSoftmaxRegs = 216, kOtherRegs = 72;
 static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * kLaunchRegs, "register shares");
 
 struct TilePlan {
+  int run;               // rows of a box: the largest power of two dividing the page, at most a tile; 0: rows one by one
   int joint;             // prefix and own keys of a request are one segment (no stacking over requests)
   int ctas;
   int64_t* start;        // [batch + 1] first tile of request i on the line
@@ -193,6 +194,12 @@ struct TilePlan {
   float* whole_lse;      // [2][tokens * hq]
   float* cut;            // [2 * ctas][kBlock][dim] rows of cut segments: CTA's first and last stretch
   float* cut_lse;        // [2 * ctas][kBlock]
+};
+
+// Tensor maps of the pool's K and V rows ([pool_rows, hk * dim], 128-byte
+// swizzle): boxes of 64 values x `run` rows, and single rows.
+struct PoolMaps {
+  CUtensorMap box[2], row[2];
 };
 
 // One segment: nrow rows from row `row0` of the row space that starts at token
@@ -204,7 +211,7 @@ struct Segment {
   int tiles;
 };
 
-__device__ __forceinline__ int tile_count(int64_t keys) { return keys <= 0 ? 1 : (int)((keys + kKeys - 1) / kKeys); }
+__device__ __forceinline__ int tile_count(int64_t keys) { return (int)((keys + kKeys - 1) / kKeys); }
 
 // The line of tiles as one thread walks it.
 struct Walk {
@@ -231,21 +238,28 @@ struct Walk {
     const int64_t x = g.len - g.ntok + j + 1;
     return x < 0 ? 0 : (x > g.len ? g.len : x);
   }
-  // Keys of the segment that its row x sees.
-  __device__ __forceinline__ int64_t seen(int x) const {
-    if (g.req < 0) return a.prefix_len;
-    return (p.joint ? a.prefix_len : 0) + own_seen((int)a.group_div.div((uint32_t)x));
+  // Own keys that row x of the segment sees.
+  __device__ __forceinline__ int64_t row_seen(int x) const {
+    return g.req < 0 ? 0 : own_seen((int)a.group_div.div((uint32_t)x));
   }
   __device__ __forceinline__ int rows() const {
     const int64_t r = (int64_t)g.ntok * a.group - (int64_t)g.blk * kBlock;
     return r < kBlock ? (int)r : kBlock;
   }
-  __device__ __forceinline__ int64_t keys() const { return seen(g.blk * kBlock + rows() - 1); }
-  __device__ __forceinline__ void size() { g.tiles = tile_count(keys()); }
+  // Own keys of the block: what its last row sees.
+  __device__ __forceinline__ int64_t own_keys() const { return row_seen(g.blk * kBlock + rows() - 1); }
+  // Prefix tiles of the segment come first; no tile holds both kinds of keys. A
+  // block without keys still has a tile, which writes its empty rows.
+  __device__ __forceinline__ int prefix_part() const { return g.req < 0 || p.joint ? tile_count(a.prefix_len) : 0; }
+  __device__ __forceinline__ int block_tiles() const {
+    const int n = prefix_part() + tile_count(own_keys());
+    return n < 1 ? 1 : n;
+  }
+  __device__ __forceinline__ void size() { g.tiles = block_tiles(); }
   // Tiles of one head of the request.
   __device__ __forceinline__ int64_t head_tiles() {
     int64_t n = 0;
-    for (g.blk = 0; g.blk < g.nblk; ++g.blk) n += tile_count(keys());
+    for (g.blk = 0; g.blk < g.nblk; ++g.blk) n += block_tiles();
     return n;
   }
   __device__ __forceinline__ void prefix_space() {
@@ -313,24 +327,88 @@ template <int DP>
 struct TileShape {
   static constexpr int tile = kRows * DP * 2;                     // bytes of a Q, K or V tile
   static constexpr int stages = DP == 128 ? 5 : 12;               // K and V tiles in flight
-  static constexpr int queue = DP == 128 ? 3 : 6;                 // loads not yet waited for
   static constexpr int data = (2 + stages) * tile;
-  static constexpr int smem = data + 2 * 2 * kRows * 4 + 512;
+  static constexpr int smem = data + 3072;
 };
 
 // Shared memory behind the tiles.
 struct TileShared {
   float m[2][kRows], l[2][kRows];   // the two warpgroups' halves of the same rows
   uint64_t full[12], empty[12], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], o_empty, halves, halves_read;
+  alignas(16) int32_t rows[kKeys];  // pool rows of the tile being loaded
   Segment first;                    // where this CTA's stretch starts
   int64_t first_off, total;
   uint32_t tmem;
   int quit;
 };
-static_assert(sizeof(TileShared) <= 2 * 2 * kRows * 4 + 512, "shared memory behind the tiles");
+static_assert(sizeof(TileShared) <= 3072, "shared memory behind the tiles");
+
+// Positions in the ring are counted in 32 bits and taken back by a multiple of
+// two turns (which keeps stage and parity) long before they overflow.
+template <int ST>
+constexpr uint32_t kTurn = (1u << 30) / (2 * ST) * (2 * ST);
+template <int ST>
+__device__ __forceinline__ uint32_t next_pos(uint32_t pos, int tiles) {
+  pos += 2 * (uint32_t)tiles;
+  return pos >= kTurn<ST> ? pos - kTurn<ST> : pos;
+}
+
+// One row's share of a tile: the scores at tensor memory `ts` (128 columns) become
+// 16-bit P there; (m, l) follow, and O at `to` (when it holds something) is
+// brought to the new reference. CUT: only the first `cols` keys are seen.
+template <typename T, int DP, bool CUT>
+__device__ __forceinline__ void softmax_tile(uint32_t ts, uint32_t to, float c, int cols, bool has_o, float& m,
+                                             float& l) {
+  uint32_t s[128];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) tc::ld32(ts + k * 32, s + k * 32);
+  tc::wait_ld();
+  float t4[4] = {m, m, m, m};
+#pragma unroll
+  for (int k = 0; k < 128; ++k)
+    if (!CUT || k < cols) t4[k & 3] = fmaxf(t4[k & 3], __uint_as_float(s[k]));
+  const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+  // move the reference when it is too far behind (or there is none yet)
+  const bool move = (top - m) * c > 8.f || (m == -INFINITY && top > -INFINITY);
+  if (__any_sync(0xffffffffu, move)) {
+    const float f = !move ? 1.f : (m == -INFINITY ? 0.f : tc::ex2((m - top) * c));
+    if (move) m = top;
+    l *= f;
+    if (has_o) {
+      uint32_t o[32];
+#pragma unroll 1
+      for (int k = 0; k < DP; k += 32) {
+        tc::ld32(to + k, o);
+        tc::wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+        tc::st32(to + k, o);
+      }
+    }
+  }
+  const float mc = m == -INFINITY ? 0.f : m * c;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int k = h * 64; k < h * 64 + 64; k += 2) {
+      float p0 = tc::ex2(fmaf(__uint_as_float(s[k]), c, -mc));
+      float p1 = tc::ex2(fmaf(__uint_as_float(s[k + 1]), c, -mc));
+      if (CUT) {
+        p0 = k < cols ? p0 : 0.f;
+        p1 = k + 1 < cols ? p1 : 0.f;
+      }
+      sum[(k >> 1) & 3] += p0 + p1;
+      s[k >> 1] = Vec16<T>::pack2(p0, p1);
+    }
+    tc::st32(ts + h * 32, s + h * 32);
+  }
+  l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const AttnArgs a, const TilePlan p) {
+__global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const AttnArgs a, const TilePlan p,
+                                                                     const __grid_constant__ PoolMaps maps) {
   using Shape = TileShape<DP>;
   constexpr int ST = Shape::stages;
   constexpr bool kBf16 = Vec16<T>::bf16;
@@ -339,11 +417,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < ST; ++i) {
-      pipe::bar_init(sh.full + i, 3);
+      pipe::bar_init(sh.full + i, 1);
       pipe::bar_init(sh.empty + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
-      pipe::bar_init(sh.q_full + i, 3);
+      pipe::bar_init(sh.q_full + i, 2);
       pipe::bar_init(sh.q_empty + i, 1);
       pipe::bar_init(sh.s_full + i, 1);
       pipe::bar_init(sh.p_full + i, 4);
@@ -371,10 +449,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
     int64_t* wsum = reinterpret_cast<int64_t*>(smem);  // the tiles' memory is not in use yet
     const int per = (a.batch + kTileThreads - 1) / kTileThreads;
     const int r0 = tid * per < a.batch ? tid * per : a.batch, r1 = r0 + per < a.batch ? r0 + per : a.batch;
-    int64_t mine = 0;
+    int64_t mine = 0, last = 0;  // tiles of the run, of one head of its last request
     for (int r = r0; r < r1; ++r) {
       w.request(r);
-      mine += w.head_tiles() * a.hk;
+      last = w.head_tiles();
+      mine += last * a.hk;
       if (blockIdx.x == 0 && (__ldg(a.lens + r) > (int64_t)a.width * a.page || __ldg(a.lens + r) < 0 ||
                               __ldg(a.cu + r) < 0 || __ldg(a.cu + r + 1) > a.tokens ||
                               __ldg(a.cu + r + 1) < __ldg(a.cu + r)))
@@ -409,8 +488,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
       }
     }
     for (int r = r0; r < r1; ++r) {
-      w.request(r);
-      const int64_t one = w.head_tiles();
+      if (per > 1) {
+        w.request(r);
+        last = w.head_tiles();
+      }
+      const int64_t one = last;
       if (blockIdx.x == 0) p.start[r] = at;
       if (x0 >= at && x0 < at + one * a.hk) {
         int64_t y = x0 - at;
@@ -453,7 +535,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
         const int rows = w.rows(), n = (int)(w.g.tiles - off < left ? w.g.tiles - off : left);
         const bool pair = rows > kRows;
         const int mine = pair ? t * kRows + r : r;             // this thread's row of the block
-        const int64_t see = mine < rows ? w.seen(w.g.blk * kBlock + mine) : 0;
+        const int np = w.prefix_part();
+        const int64_t see = mine < rows ? w.row_seen(w.g.blk * kBlock + mine) : 0;
         const bool warp_on = __any_sync(0xffffffffu, mine < rows);
         float m = -INFINITY, l = 0.f;
         bool ok = true;
@@ -463,58 +546,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
           ++n_s;
           tc::fence_after();
           if (warp_on) {
-            uint32_t s[128];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) tc::ld32(ts + k * 32, s + k * 32);
-            tc::wait_ld();
-            const int64_t rest = see - (int64_t)(off + i) * kKeys;
+            const int ti = off + i;
+            const int64_t rest = ti >= np ? see - (int64_t)(ti - np) * kKeys
+                                          : (mine < rows ? a.prefix_len - ti * kKeys : 0);
             const int cols = rest < 0 ? 0 : (rest < kKeys ? (int)rest : kKeys);
-            const bool cut = __any_sync(0xffffffffu, cols < kKeys);
-            float top = m;
-            if (cut) {
-#pragma unroll
-              for (int k = 0; k < 128; ++k)
-                if (k < cols) top = fmaxf(top, __uint_as_float(s[k]));
-            } else {
-              float t4[4] = {m, m, m, m};
-#pragma unroll
-              for (int k = 0; k < 128; ++k) t4[k & 3] = fmaxf(t4[k & 3], __uint_as_float(s[k]));
-              top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-            }
-            // move the reference when it is too far behind (or there is none yet)
-            const bool move = (top - m) * c > 8.f || (m == -INFINITY && top > -INFINITY);
-            if (__any_sync(0xffffffffu, move)) {
-              const float f = !move ? 1.f : (m == -INFINITY ? 0.f : tc::ex2((m - top) * c));
-              if (move) m = top;
-              l *= f;
-              if (i >= 2 || (pair && i > 0)) {  // O holds something
-                uint32_t o[32];
-#pragma unroll 1
-                for (int k = 0; k < DP; k += 32) {
-                  tc::ld32(to + k, o);
-                  tc::wait_ld();
-#pragma unroll
-                  for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                  tc::st32(to + k, o);
-                }
-              }
-            }
-            const float mc = m == -INFINITY ? 0.f : m * c;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < 128; k += 2) {
-              float p0 = tc::ex2(fmaf(__uint_as_float(s[k]), c, -mc));
-              float p1 = tc::ex2(fmaf(__uint_as_float(s[k + 1]), c, -mc));
-              if (cut) {
-                p0 = k < cols ? p0 : 0.f;
-                p1 = k + 1 < cols ? p1 : 0.f;
-              }
-              sum[(k >> 1) & 3] += p0 + p1;
-              s[k >> 1] = Vec16<T>::pack2(p0, p1);
-            }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tc::st32(ts, s);
-            tc::st32(ts + 32, s + 32);
+            const bool has_o = pair ? i > 0 : i >= 2;
+            if (__any_sync(0xffffffffu, cols < kKeys))
+              softmax_tile<T, DP, true>(ts, to, c, cols, has_o, m, l);
+            else
+              softmax_tile<T, DP, false>(ts, to, c, cols, has_o, m, l);
             tc::wait_st();
           }
           tc::fence_before();
@@ -613,179 +653,200 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
     tc::regs_down<kOtherRegs>();
     if (warp == 8) {
       // -------------------------------------------------------- products ----
-      if (lane == 0) {
-        const uint32_t id_s = tc::idesc(kBf16, kRows, kKeys, false, a.scale < 0.f);
-        const uint32_t id_o = tc::idesc(kBf16, kRows, (a.dim + 15) / 16 * 16, true);
-        const int ks = (a.dim + 15) / 16;
-        const uint32_t base = tc::smem_addr(smem), ring = base + 2 * Shape::tile;
-        uint32_t n_p[2] = {0, 0}, n_piece = 0, n_q = 0;
-        int64_t pos = 0;
-        bool ok = true;
-        while (ok) {
-          const int rows = w.rows(), n = (int)(w.g.tiles - off < left ? w.g.tiles - off : left);
-          const bool pair = rows > kRows;
-          const int nq = pair ? 2 : 1;
-          for (int b = 0; b < nq && ok; ++b)
-            ok = wait_or_quit(sh.q_full + ((n_q + b) & 1), ((n_q + b) >> 1) & 1, quit);
-          if (!ok) break;
-          const uint32_t q0 = base + (n_q & 1) * Shape::tile, q1 = pair ? base + ((n_q + 1) & 1) * Shape::tile : q0;
-          const auto tile_of = [&](int k, int t) { return pair ? k : 2 * k + t; };
-          const auto scores = [&](int k, int t) {
-            const int i = tile_of(k, t);
-            if (i >= n) return true;
-            const int64_t at = pos + 2 * (int64_t)i;
-            const int st = (int)(at % ST);
-            if (!wait_or_quit(sh.full + st, (uint32_t)(at / ST) & 1, quit)) return false;
-            tc::fence_after();
-            const uint32_t q = t ? q1 : q0, kt = ring + st * Shape::tile;
-            for (int j = 0; j < ks; ++j) {
-              const uint32_t o = (j >> 2) * (kRows * 128) + (j & 3) * 32;
-              tc::mma_ss(tmem + t * 128, tc::desc(q + o, 16, 1024), tc::desc(kt + o, 16, 1024), id_s, j > 0);
+      // The whole warp walks along; one lane issues.
+      const uint32_t id_s = tc::idesc(kBf16, kRows, kKeys, false, a.scale < 0.f);
+      const uint32_t id_o = tc::idesc(kBf16, kRows, a.dim, true);
+      const int ks = a.dim / 16;
+      const uint32_t base = tc::smem_addr(smem), ring = base + 2 * Shape::tile;
+      uint32_t n_p[2] = {0, 0}, n_piece = 0, n_q = 0;
+      uint32_t pos = 0;  // counts K and V tiles, modulo 2^32 in whole turns of the ring
+      bool ok = true;
+      while (ok) {
+        const int rows = w.rows(), n = (int)(w.g.tiles - off < left ? w.g.tiles - off : left);
+        const bool pair = rows > kRows;
+        const int nq = pair ? 2 : 1;
+        for (int b = 0; b < nq && ok; ++b)
+          ok = warp_wait(sh.q_full + ((n_q + b) & 1), ((n_q + b) >> 1) & 1, quit);
+        if (!ok) break;
+        const uint32_t q0 = base + (n_q & 1) * Shape::tile, q1 = pair ? base + ((n_q + 1) & 1) * Shape::tile : q0;
+        const auto tile_of = [&](int k, int t) { return pair ? k : 2 * k + t; };
+        const auto scores = [&](int k, int t) {
+          const int i = tile_of(k, t);
+          if (i >= n) return true;
+          const uint32_t at = pos + 2 * (uint32_t)i, st = at % ST;
+          if (!warp_wait(sh.full + st, (at / ST) & 1, quit)) return false;
+          tc::fence_after();
+          const uint64_t qd = tc::desc(t ? q1 : q0, 16, 1024), kd = tc::desc(ring + st * Shape::tile, 16, 1024);
+          if (tc::elect()) {
+#pragma unroll
+            for (int j = 0; j < DP / 16; ++j) {
+              const uint32_t o = ((j >> 2) * (kRows * 128) + (j & 3) * 32) >> 4;
+              if (j < ks) tc::mma_ss(tmem + t * 128, qd + o, kd + o, id_s, j > 0);
             }
             tc::commit(sh.s_full + t);
             if (!pair || t == 1) tc::commit(sh.empty + st);
-            return true;
-          };
-          ok = scores(0, 0) && scores(0, 1);
-          for (int k = 0; ok && tile_of(k, 0) < n; ++k) {
-            for (int t = 0; ok && t < 2; ++t) {
-              const int i = tile_of(k, t);
-              if (i >= n) break;
-              ok = wait_or_quit(sh.p_full + t, n_p[t] & 1, quit);
-              if (!ok) break;
-              ++n_p[t];
-              if (k == 0 && t == 0 && n_piece > 0 && !(ok = wait_or_quit(&sh.o_empty, (n_piece - 1) & 1, quit))) break;
-              const int64_t at = pos + 2 * (int64_t)i + 1;
-              const int st = (int)(at % ST);
-              if (!(ok = wait_or_quit(sh.full + st, (uint32_t)(at / ST) & 1, quit))) break;
-              tc::fence_after();
-              const uint32_t vt = ring + st * Shape::tile;
+          }
+          __syncwarp();
+          return true;
+        };
+        ok = scores(0, 0) && scores(0, 1);
+        for (int k = 0; ok && tile_of(k, 0) < n; ++k) {
+          for (int t = 0; ok && t < 2; ++t) {
+            const int i = tile_of(k, t);
+            if (i >= n) break;
+            const uint32_t at = pos + 2 * (uint32_t)i + 1, st = at % ST;
+            ok = warp_wait(sh.full + st, (at / ST) & 1, quit) && warp_wait(sh.p_full + t, n_p[t] & 1, quit);
+            if (!ok) break;
+            ++n_p[t];
+            if (k == 0 && t == 0 && n_piece > 0 && !(ok = warp_wait(&sh.o_empty, (n_piece - 1) & 1, quit))) break;
+            tc::fence_after();
+            const uint64_t vd = tc::desc(ring + st * Shape::tile, kKeys * 128, 1024);
+            if (tc::elect()) {
+#pragma unroll
               for (int j = 0; j < kKeys / 16; ++j)
-                tc::mma_ts(tmem + 256 + t * 128, tmem + t * 128 + j * 8,
-                           tc::desc(vt + j * 2048, kKeys * 128, 1024), id_o, k > 0 || j > 0);
+                tc::mma_ts(tmem + 256 + t * 128, tmem + t * 128 + j * 8, vd + ((j * 2048) >> 4), id_o, k > 0 || j > 0);
               if (!pair || t == 1) tc::commit(sh.empty + st);
               if (tile_of(k + 1, t) >= n) tc::commit(sh.o_full + t);
-              ok = scores(k + 1, t);
             }
+            __syncwarp();
+            ok = scores(k + 1, t);
           }
-          if (!ok) break;
+        }
+        if (!ok) break;
+        if (tc::elect())
           for (int b = 0; b < nq; ++b) tc::commit(sh.q_empty + ((n_q + b) & 1));
-          n_q += nq;
-          pos += 2 * (int64_t)n;
-          ++n_piece;
+        __syncwarp();
+        n_q += nq;
+        pos = next_pos<ST>(pos, n);
+        ++n_piece;
+        left -= n;
+        if (left <= 0) break;
+        off = 0;
+        w.next();
+      }
+    } else {
+      // ----------------------------------------------------------- loads ----
+      constexpr int CH = DP / 8, PN = DP / 64;                  // 16-byte chunks and 64-value panels of a row
+      constexpr uint32_t kPanel = kRows * 128;
+      const uint32_t base = tc::smem_addr(smem), ring = base + 2 * Shape::tile;
+      if (warp == 9) {
+        // keys and values: whole pages as boxes; a tile with a page that is cut
+        // short, or outside the pool, row by row, four rows at a time, with zeros
+        // for what is not there (a slot behind the end may hold anything)
+        if (lane < 2) {
+          tc::prefetch_map(maps.box + lane);
+          tc::prefetch_map(maps.row + lane);
+        }
+        const int none = (int)a.pool_rows;                      // a row outside the map
+        uint32_t pos = 0;
+        bool ok = true;
+        while (ok) {
+          const int n = (int)(w.g.tiles - off < left ? w.g.tiles - off : left);
+          const int np = w.prefix_part();
+          const int64_t own = w.own_keys();
+          for (int i = 0; i < n && ok; ++i) {
+            const int ti = off + i;
+            const bool pre = ti < np;
+            const int64_t key0 = (int64_t)(pre ? ti : ti - np) * kKeys;
+            const int64_t rest = (pre ? a.prefix_len : own) - key0;
+            const int valid = rest < 0 ? 0 : (rest < kKeys ? (int)rest : kKeys);
+            const int shift = pre ? 0 : a.prefix_len;           // own keys follow the prefix
+            bool boxes = p.run > 0 && valid == kKeys;
+            if (boxes) {
+              int32_t y = 0;
+              if (lane * p.run < kKeys) {
+                const int64_t sl = key_slot(a, w.g.req, (int32_t)key0 + lane * p.run + shift);
+                y = sl < 0 || sl + p.run > a.pool_rows ? -1 : (int32_t)sl;
+                sh.rows[lane] = y;
+              }
+              boxes = !__any_sync(0xffffffffu, y < 0);
+            }
+            if (!boxes) {
+              int4 y = make_int4(none, none, none, none);
+              int32_t* e = &y.x;
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (lane * 4 + j < valid) {
+                  const int64_t sl = key_slot(a, w.g.req, (int32_t)key0 + lane * 4 + j + shift);
+                  if (sl >= 0) e[j] = (int32_t)sl;
+                }
+              *reinterpret_cast<int4*>(sh.rows + lane * 4) = y;
+            }
+            __syncwarp();
+            for (int kv = 0; kv < 2; ++kv, ++pos) {
+              const uint32_t st = pos % ST;
+              if (pos >= ST && !(ok = warp_wait(sh.empty + st, (pos / ST - 1) & 1, quit))) break;
+              if (tc::elect()) {
+                pipe::bar_expect_tx(sh.full + st, Shape::tile);
+                const uint32_t dst = ring + st * Shape::tile;
+                const int x = w.g.kh * a.dim;
+                if (boxes) {
+                  const int nb = kKeys / p.run;
+#pragma unroll 2
+                  for (int b = 0; b < nb; ++b) {
+                    const int y = sh.rows[b];
+#pragma unroll
+                    for (int pn = 0; pn < PN; ++pn)
+                      tc::load_box(dst + pn * kPanel + b * p.run * 128, maps.box + kv, x + pn * 64, y, sh.full + st);
+                  }
+                } else {
+#pragma unroll 2
+                  for (int b = 0; b < kKeys / 4; ++b) {
+                    const int4 y = *reinterpret_cast<const int4*>(sh.rows + b * 4);
+#pragma unroll
+                    for (int pn = 0; pn < PN; ++pn)
+                      tc::load_rows(dst + pn * kPanel + b * 512, maps.row + kv, x + pn * 64, y, sh.full + st);
+                  }
+                }
+              }
+              __syncwarp();
+            }
+            if (pos >= kTurn<ST>) pos -= kTurn<ST> - ST * 2;  // keeps stage and parity, and counts as a full ring
+          }
+          left -= n;
+          if (left <= 0) break;
+          off = 0;
+          w.next();
+        }
+        // copies must not outlive the CTA: all are waited for by the products, unless a wait gave up
+        if (*quit)
+          for (uint32_t q = pos > ST ? pos - ST : 0; q < pos; ++q) (void)pipe::bar_wait(sh.full + q % ST, (q / ST) & 1);
+      } else {
+        // queries: only the rows that exist (a product's rows do not mix)
+        constexpr int RI = 32 / CH;                             // rows per instruction
+        const int lw = warp - 10, ch = lane % CH, sub = lane / CH;
+        const bool in_dim = ch * 8 < a.dim;
+        const uint32_t panel = (uint32_t)(ch >> 3) * kPanel;
+        uint32_t n_q = 0;
+        bool ok = true;
+        while (ok) {
+          const int rows = w.rows(), n = (int)(w.g.tiles - off < left ? w.g.tiles - off : left);
+          const int nq = rows > kRows ? 2 : 1;
+          for (int b = 0; b < nq; ++b, ++n_q) {
+            const int buf = n_q & 1;
+            if (n_q >= 2 && !(ok = warp_wait(sh.q_empty + buf, ((n_q >> 1) - 1) & 1, quit))) break;
+            const uint32_t dst = base + buf * Shape::tile;
+            const int here = rows - b * kRows < kRows ? rows - b * kRows : kRows;
+#pragma unroll 4
+            for (int rr = lw * RI + sub; rr < here; rr += 2 * RI) {
+              const int x = w.g.blk * kBlock + b * kRows + rr;
+              const int jt = (int)a.group_div.div((uint32_t)x);
+              const char* src = a.q + ((int64_t)w.g.tok + jt) * a.q_pitch +
+                                (int64_t)(w.g.kh * a.group + x - jt * a.group) * a.q_head + ch * 16;
+              if (in_dim) tc::copy16(dst + panel + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4), src, true);
+            }
+            tc::copy_commit();
+            tc::copy_wait<0>();
+            tc::fence_async();
+            __syncwarp();
+            if (lane == 0) pipe::bar_arrive(sh.q_full + buf);
+          }
           left -= n;
           if (left <= 0) break;
           off = 0;
           w.next();
         }
       }
-      __syncwarp();
-    } else {
-      // ----------------------------------------------------------- loads ----
-      constexpr int CH = DP / 8, RI = 32 / CH;                  // 16-byte chunks of a row; rows per instruction
-      constexpr int IT = (kRows / RI + 2) / 3;                  // instructions per warp and tile
-      const int lw = warp - 9, ch = lane % CH, sub = lane / CH;
-      const bool in_dim = ch * 8 < a.dim;
-      const uint32_t base = tc::smem_addr(smem), ring = base + 2 * Shape::tile;
-      const uint32_t panel = (uint32_t)(ch >> 3) * (kRows * 128);
-      uint64_t* queue[Shape::queue] = {};
-      int queued = 0;
-      // loads are announced once they have landed: the oldest when the queue is
-      // full, all of them before a wait for a free stage
-      const auto announce = [&](uint64_t* bar) {
-        tc::fence_async();
-        __syncwarp();
-        if (lane == 0) pipe::bar_arrive(bar);
-      };
-      const auto push = [&](uint64_t* bar) {
-        tc::copy_commit();
-        if (queued == Shape::queue) {
-          tc::copy_wait<Shape::queue>();
-          announce(queue[0]);
-#pragma unroll
-          for (int i = 0; i + 1 < Shape::queue; ++i) queue[i] = queue[i + 1];
-          queue[Shape::queue - 1] = bar;
-        } else {
-#pragma unroll
-          for (int i = 0; i < Shape::queue; ++i)
-            if (i == queued) queue[i] = bar;
-          ++queued;
-        }
-      };
-      const auto flush = [&]() {
-        tc::copy_wait<0>();
-#pragma unroll
-        for (int i = 0; i < Shape::queue; ++i)
-          if (i < queued) announce(queue[i]);
-        queued = 0;
-      };
-      const auto acquire = [&](uint64_t* bar, uint32_t parity) {
-        bool free = pipe::bar_try(bar, parity);
-        free = __all_sync(0xffffffffu, free);
-        if (free) return true;
-        flush();
-        return warp_wait(bar, parity, quit);
-      };
-      uint32_t n_q = 0;
-      int64_t pos = 0;
-      bool ok = true;
-      while (ok) {
-        const int rows = w.rows(), n = (int)(w.g.tiles - off < left ? w.g.tiles - off : left);
-        const int nq = rows > kRows ? 2 : 1;
-        for (int b = 0; b < nq && ok; ++b, ++n_q) {
-          const int buf = n_q & 1;
-          if (n_q >= 2 && !(ok = acquire(sh.q_empty + buf, ((n_q >> 1) - 1) & 1))) break;
-          const uint32_t dst = base + buf * Shape::tile;
-#pragma unroll 4
-          for (int it = 0; it < IT; ++it) {
-            const int gi = lw + 3 * it, rr = gi * RI + sub;
-            if (gi * RI >= kRows) break;
-            const int br = b * kRows + rr, x = w.g.blk * kBlock + br;
-            const bool valid = in_dim && br < rows;
-            const int jt = valid ? (int)a.group_div.div((uint32_t)x) : 0;
-            const char* src = a.q;
-            if (valid)
-              src += ((int64_t)w.g.tok + jt) * a.q_pitch + (int64_t)(w.g.kh * a.group + x - jt * a.group) * a.q_head + ch * 16;
-            tc::copy16(dst + panel + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4), src, valid);
-          }
-          push(sh.q_full + buf);
-        }
-        const int64_t keys = w.g.req < 0 ? a.prefix_len : w.keys();
-        const int shift = w.g.req < 0 || p.joint ? 0 : a.prefix_len;
-        const int head = w.g.kh * a.dim * 2;
-        for (int i = 0; i < n && ok; ++i) {
-          // slots of this warp's rows: two per lane
-          int32_t slot[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int q = lane + 32 * u, rr = (lw + 3 * (q / RI)) * RI + q % RI;
-            const int64_t x = (int64_t)(off + i) * kKeys + rr;
-            slot[u] = rr < kRows && x < keys ? (int32_t)key_slot(a, w.g.req, (int32_t)x + shift) : -1;
-          }
-          for (int kv = 0; kv < 2; ++kv, ++pos) {
-            const int st = (int)(pos % ST);
-            if (pos >= ST && !(ok = acquire(sh.empty + st, (uint32_t)(pos / ST - 1) & 1))) break;
-            const uint32_t dst = ring + st * Shape::tile;
-            const char* from = a.pool + (kv ? a.plane : 0) + head + ch * 16;
-#pragma unroll
-            for (int it = 0; it < IT; ++it) {
-              const int gi = lw + 3 * it, rr = gi * RI + sub, q = it * RI + sub;
-              const int32_t sl = __shfl_sync(0xffffffffu, q < 32 ? slot[0] : slot[1], q & 31);
-              if (gi * RI < kRows) {
-                const bool valid = in_dim && sl >= 0;
-                tc::copy16(dst + panel + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4),
-                           valid ? from + (int64_t)sl * a.pitch : a.pool, valid);
-              }
-            }
-            push(sh.full + st);
-          }
-        }
-        left -= n;
-        if (left <= 0) break;
-        off = 0;
-        w.next();
-      }
-      flush();
     }
     }
   }
@@ -855,7 +916,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttnArgs a, cons
       int64_t before = 0, one = 0, here = 0;  // tiles of the blocks before this one, of all, of this one
       for (int b = lane; b < w.g.nblk; b += 32) {
         w.g.blk = b;
-        const int n = tile_count(w.keys());
+        const int n = w.block_tiles();
         one += n;
         if (b < blk) before += n;
         if (b == blk) here = n;
@@ -937,10 +998,10 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttnArgs a, cons
   if (lane == 0 && a.lse) a.lse[grow] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
-// The tensor core takes 16-bit values; a head of more than 128 of them, or of
-// 32-bit values, goes row by row.
+// The tensor core takes 16-bit values, sixteen at a time; a head of more than
+// 128 of them, of an odd half of sixteen, or of 32-bit values goes row by row.
 bool takes_tiles(const AttnArgs& a, int dtype) {
-  return dtype != GSEC_F32 && a.dim <= 128 && a.pool_rows < (1ll << 31);
+  return dtype != GSEC_F32 && a.dim <= 128 && a.dim % 16 == 0;
 }
 
 // Stacking the requests' rows over the prefix pays when they would not fill
@@ -949,6 +1010,8 @@ bool takes_tiles(const AttnArgs& a, int dtype) {
 TilePlan tile_plan(const AttnArgs& a, int64_t* bytes) {
   TilePlan p{};
   p.ctas = sm_count();
+  p.run = a.page & -a.page;  // boxes start at pages, tiles at multiples of 128 keys
+  p.run = p.run < 8 ? 0 : (p.run > kKeys ? kKeys : p.run);
   p.joint = a.prefix_len == 0 || a.batch == 1 || a.tokens * a.group >= (int64_t)a.batch * kRows;
   char* at = a.workspace;
   const auto take = [&](int64_t n) {
@@ -966,10 +1029,50 @@ TilePlan tile_plan(const AttnArgs& a, int64_t* bytes) {
   return p;
 }
 
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The driver's encoder of tensor maps, or null.
+EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) !=
+            cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeTiled>(f);
+  }();
+  return fn;
+}
+
+bool pool_map(CUtensorMap* m, bool bf16, const char* at, int64_t values, int64_t rows, int64_t pitch, int box_rows) {
+  const cuuint64_t size[2] = {(cuuint64_t)values, (cuuint64_t)rows}, stride[1] = {(cuuint64_t)pitch};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, step[2] = {1, 1};
+  const EncodeTiled encode = encode_tiled();
+  return encode != nullptr &&
+         encode(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                const_cast<char*>(at), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int DP>
 int launch_tiles(const AttnArgs& a, cudaStream_t s) {
   int64_t bytes = 0;
   const TilePlan p = tile_plan(a, &bytes);
+  PoolMaps maps;
+  bool ok = true;
+  for (int kv = 0; kv < 2; ++kv) {
+    const char* at = a.pool + (kv ? a.plane : 0);
+    ok = ok && pool_map(maps.box + kv, Vec16<T>::bf16, at, (int64_t)a.hk * a.dim, a.pool_rows, a.pitch, p.run ? p.run : 1) &&
+         pool_map(maps.row + kv, Vec16<T>::bf16, at, (int64_t)a.hk * a.dim, a.pool_rows, a.pitch, 1);
+  }
+  if (!ok) {
+    set_error("prefix_attention: the pool's tensor maps were refused");
+    return GSEC_ECUDA;
+  }
   constexpr int smem = TileShape<DP>::smem;
   if (launch_cache().blocks_per_sm(attend_tile_kernel<T, DP>, kTileThreads, smem) < 0)
     return check_launch("attend_tile launch shape");
@@ -979,7 +1082,7 @@ int launch_tiles(const AttnArgs& a, cudaStream_t s) {
     return cudaFuncGetAttributes(&at, attend_tile_kernel<T, DP>) == cudaSuccess && at.numRegs == kLaunchRegs;
   }();
   GSEC_REQUIRE(regs_ok, "attend_tile: launch registers are not %d", kLaunchRegs);
-  const int rc = launch_rc(launch_pdl(attend_tile_kernel<T, DP>, dim3((unsigned)p.ctas), dim3(kTileThreads), smem, s, a, p),
+  const int rc = launch_rc(launch_pdl(attend_tile_kernel<T, DP>, dim3((unsigned)p.ctas), dim3(kTileThreads), smem, s, a, p, maps),
                            "prefix_attention");
   if (rc) return rc;
   const int64_t rows = a.tokens * a.hq;

@@ -2,6 +2,7 @@
 // matrix instructions and their commits, and 16-byte asynchronous copies.
 #pragma once
 
+#include <cuda.h>
 #include <stdint.h>
 
 #include "pipe.cuh"
@@ -10,6 +11,16 @@ namespace gsec {
 namespace tc {
 
 using pipe::smem_addr;
+
+// One lane of a whole warp, the same every time. Matrix instructions, tensor
+// copies and commits take their operands from registers that a warp shares: under
+// any other condition the compiler issues them lane by lane (measured: about 95
+// cycles per copy and 190 per product instead of a few).
+__device__ __forceinline__ bool elect() {
+  uint32_t on;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(on));
+  return on != 0;
+}
 
 // ------------------------------------------------------------ tensor memory --
 // 512 columns x 128 lanes x 32 bits per SM; an address is lane << 16 | column.
@@ -101,6 +112,24 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 template <int N>
 __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// Box of a two-dimensional tensor map at (x, y), completing on `bar`.
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar))
+      : "memory");
+}
+// Four rows of a tensor map (box one row high), one after the other; a row outside the map is zeros.
+__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, int x, const int4& y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w), "r"(smem_addr(bar))
+      : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 // Ordinary writes to shared memory before, reads by the tensor core after.
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
