@@ -677,6 +677,7 @@ int gsec_prefix_attention_workspace(int64_t tokens, int32_t batch, int64_t prefi
   a.hk = hk;
   a.group = hq / hk;
   a.dim = dim;
+  a.scale = 1.f;  // any that is not next to nothing: those need no workspace
   *bytes = attention_workspace(a, dtype);
   return GSEC_OK;
 }

@@ -170,30 +170,62 @@ int attend_rows(const AttnArgs& a, cudaStream_t s) {
 // well as they hold 1.
 //
 // Two warpgroups take turns, so that one's exponentials run under the other's
-// products: with more than 128 rows in the block each has its own 128 rows and
-// both see every tile; otherwise they take the even and the odd tiles of the
-// same rows and add up their halves at the end.
+// products. A tile of a block with more than 128 rows is two steps, one for each
+// half of the rows; otherwise it is one. Steps go to the warpgroups in turn
+// without a break between segments; a block of one half with several tiles has
+// its even and its odd tiles in different hands, which are added up at its end.
 //
-// Work is dealt out evenly whatever the lengths: all tiles of all segments form
-// one line, and each of the resident CTAs takes an equal stretch of it. A segment
-// cut by a stretch's end, and the two halves (prefix, own keys) of a row, are
-// joined by attend_join_kernel from fp32 partial results and their log sums.
-constexpr int kTileThreads = 384;   // 2 softmax warpgroups; 1 issuing warp, 3 loading warps
+// Work is dealt out evenly whatever the lengths: the segments form one line,
+// measured in units of about what a step costs, and each of the resident CTAs
+// takes an equal stretch of it. A segment cut by a stretch's end, and the two
+// segments (prefix, own keys) of a row, are joined by a second kernel from fp32
+// partial results and their log sums.
+//
+// The code of a warp that meets a new path comes from L2 at some hundred cycles
+// a line, and a segment of one tile takes every path once: the walk along the
+// line is one warp's work, which hands the pieces to the others through shared
+// memory, and loops are unrolled only as far as they have to be (with the walk in
+// every role and 128-column bodies a one-tile segment took 12000 cycles).
+constexpr int kTileThreads = 384;   // 2 softmax warpgroups; issue products, load K, load V, walk and load Q: a warp each
 constexpr int kRows = 128, kKeys = 128, kBlock = 256;
-// Registers: a softmax thread holds a row of 128 scores. The launch has 168 per
-// thread; the third warpgroup hands over what it does not need.
-constexpr int kLaunchRegs = 168, kSoftmaxRegs = 216, kOtherRegs = 72;
-static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * kLaunchRegs, "register shares");
+// Units of the line: a tile of a whole block; half a block's tile is three
+// quarters of that; a segment's beginning and end.
+constexpr int kUnitTile = 32, kUnitSegment = 16;
+constexpr int kMinShare = 64;       // a stretch is at least about two tiles
+
+// A block and its keys: rows [blk * kBlock, ...) of the row space that starts at
+// token `tok`; row x of it is token tok + x / group, head kh * group + x % group.
+struct Segment {
+  int req;               // request, -1: all requests over the prefix
+  int tok, ntok, len;    // query tokens of the row space; the request's own keys
+  int kh, blk, nblk;
+  int tiles;
+};
+
+struct Start {           // a point on the line
+  Segment g;
+  int y;                 // units into the segment
+};
 
 struct TilePlan {
   int run;               // rows of a box: the largest power of two dividing the page, at most a tile; 0: rows one by one
   int joint;             // prefix and own keys of a request are one segment (no stacking over requests)
   int ctas;
-  int64_t* start;        // [batch + 1] first tile of request i on the line
-  float* whole;          // [2][tokens * hq][dim] rows of uncut segments (prefix, own) that have another part
+  // rows of uncut segments (0 prefix, 1 own) that have another part
+  float* whole;          // [2][tokens * hq][dim]
   float* whole_lse;      // [2][tokens * hq]
-  float* cut;            // [2 * ctas][kBlock][dim] rows of cut segments: CTA's first and last stretch
+  int2* place;           // [2][tokens * hq] where the parts are: (-1, -1) whole, (first CTA | row << 16, last CTA)
+  // rows of cut segments: slot 2 c holds the one that goes on at the start of CTA c's stretch, 2 c + 1 the one
+  // that begins in it and goes on behind its end
+  float* cut;            // [2 * ctas][kBlock][dim]
   float* cut_lse;        // [2 * ctas][kBlock]
+  int32_t* used;         // [2 * ctas] whether the slot holds something
+  struct CutEnd* end;    // [ctas] the cut segment that ends in CTA c's stretch, if it is all its rows have
+};
+
+// Rows [x0, x0 + nrow) of the row space at token `tok`, parts with CTAs c0 .. c.
+struct CutEnd {
+  int nrow, c0, tok, kh, x0;
 };
 
 // Tensor maps of the pool's K and V rows ([pool_rows, hk * dim], 128-byte
@@ -202,18 +234,14 @@ struct PoolMaps {
   CUtensorMap box[2], row[2];
 };
 
-// One segment: nrow rows from row `row0` of the row space that starts at token
-// `tok`; row x is token tok + x / group, head kh * group + x % group.
-struct Segment {
-  int req;               // request, -1: prefix of all
-  int tok, ntok, kh, blk, nblk, own;
-  int64_t len;
-  int tiles;
-};
+__device__ __forceinline__ int tile_count(int keys) { return (keys + kKeys - 1) / kKeys; }
 
-__device__ __forceinline__ int tile_count(int64_t keys) { return (int)((keys + kKeys - 1) / kKeys); }
+__device__ __forceinline__ int live_tokens(const AttnArgs& a) {
+  const int n = __ldg(a.cu + a.batch);
+  return n < 0 ? 0 : (n > a.tokens ? (int)a.tokens : n);
+}
 
-// The line of tiles as one thread walks it.
+// The line as a thread walks it.
 struct Walk {
   const AttnArgs& a;
   const TilePlan& p;
@@ -221,66 +249,108 @@ struct Walk {
   Segment g;
   __device__ __forceinline__ Walk(const AttnArgs& a_, const TilePlan& p_, int live_) : a(a_), p(p_), live(live_) {}
 
-  __device__ __forceinline__ int prefix_keys() const { return p.joint ? 0 : a.prefix_len; }
-  // Query tokens [tok, tok + ntok) and own keys of request r, cut to what exists.
+  __device__ __forceinline__ int blocks() const { return (int)(((uint32_t)g.ntok * a.group + kBlock - 1) / kBlock); }
+  // Query tokens and own keys of request r, cut to what exists.
   __device__ __forceinline__ void request(int r) {
-    const int c0 = __ldg(a.cu + r), c1 = __ldg(a.cu + r + 1);
+    const int c0 = __ldg(a.cu + r), c1 = __ldg(a.cu + r + 1), n = __ldg(a.lens + r);
     const int lo = c0 < 0 ? 0 : (c0 > live ? live : c0), hi = c1 < lo ? lo : (c1 > live ? live : c1);
-    const int64_t room = (int64_t)a.width * a.page, n = __ldg(a.lens + r);
+    const int room = a.width * a.page;
     g.req = r;
     g.tok = lo;
     g.ntok = hi - lo;
     g.len = n < 0 ? 0 : (n > room ? room : n);
-    g.nblk = (int)(((int64_t)g.ntok * a.group + kBlock - 1) / kBlock);
+    g.nblk = blocks();
   }
-  // Own keys that token j of the request sees.
-  __device__ __forceinline__ int64_t own_seen(int j) const {
-    const int64_t x = g.len - g.ntok + j + 1;
-    return x < 0 ? 0 : (x > g.len ? g.len : x);
+  // Whether request r's numbers did not have to be cut.
+  __device__ __forceinline__ bool fits(int r) const {
+    const int c0 = __ldg(a.cu + r), c1 = __ldg(a.cu + r + 1);
+    return c0 >= 0 && c1 >= c0 && c1 <= a.tokens && __ldg(a.lens + r) == g.len;
   }
-  // Own keys that row x of the segment sees.
-  __device__ __forceinline__ int64_t row_seen(int x) const {
-    return g.req < 0 ? 0 : own_seen((int)a.group_div.div((uint32_t)x));
-  }
-  __device__ __forceinline__ int rows() const {
-    const int64_t r = (int64_t)g.ntok * a.group - (int64_t)g.blk * kBlock;
-    return r < kBlock ? (int)r : kBlock;
-  }
-  // Own keys of the block: what its last row sees.
-  __device__ __forceinline__ int64_t own_keys() const { return row_seen(g.blk * kBlock + rows() - 1); }
-  // Prefix tiles of the segment come first; no tile holds both kinds of keys. A
-  // block without keys still has a tile, which writes its empty rows.
-  __device__ __forceinline__ int prefix_part() const { return g.req < 0 || p.joint ? tile_count(a.prefix_len) : 0; }
-  __device__ __forceinline__ int block_tiles() const {
-    const int n = prefix_part() + tile_count(own_keys());
-    return n < 1 ? 1 : n;
-  }
-  __device__ __forceinline__ void size() { g.tiles = block_tiles(); }
-  // Tiles of one head of the request.
-  __device__ __forceinline__ int64_t head_tiles() {
-    int64_t n = 0;
-    for (g.blk = 0; g.blk < g.nblk; ++g.blk) n += block_tiles();
-    return n;
-  }
-  __device__ __forceinline__ void prefix_space() {
+  __device__ __forceinline__ void prefix() {
     g.req = -1;
     g.tok = 0;
     g.ntok = live;
     g.len = 0;
-    g.nblk = (int)(((int64_t)live * a.group + kBlock - 1) / kBlock);
+    g.nblk = blocks();
+  }
+  // Own keys that row x of the row space sees.
+  __device__ __forceinline__ int row_seen(int x) const {
+    if (g.req < 0) return 0;
+    const int k = g.len - g.ntok + (int)a.group_div.div((uint32_t)x) + 1;
+    return k < 0 ? 0 : (k > g.len ? g.len : k);
+  }
+  __device__ __forceinline__ int rows() const {
+    const int r = g.ntok * a.group - g.blk * kBlock;
+    return r < kBlock ? r : kBlock;
+  }
+  __device__ __forceinline__ bool pair() const { return rows() > kRows; }
+  // Own keys of the block: what its last row sees.
+  __device__ __forceinline__ int own_keys() const { return row_seen(g.blk * kBlock + rows() - 1); }
+  // Prefix tiles of the segment come first; no tile holds both kinds of keys. A
+  // block without keys still has a tile, which writes its empty rows.
+  __device__ __forceinline__ int prefix_part() const { return g.req < 0 || p.joint ? tile_count(a.prefix_len) : 0; }
+  __device__ __forceinline__ void size() {
+    const int n = prefix_part() + tile_count(own_keys());
+    g.tiles = n < 1 ? 1 : n;
+  }
+  // Units of the segment and of the first m (whole) blocks of a head. A block's
+  // own keys grow by 256 / group tokens from one to the next; taken as a straight
+  // line, the sums have a closed form, and where the line is off the true count
+  // only the balance is.
+  __device__ __forceinline__ int base_units() const {
+    const int more = g.len - g.ntok;
+    return prefix_part() * kUnitTile + (more > 0 ? more / (kKeys / kUnitTile) : 0);
+  }
+  __device__ __forceinline__ int slope() const {
+    const int s = kBlock / (kKeys / kUnitTile) / a.group;
+    return g.req < 0 ? 0 : (s > 0 ? s : 1);
+  }
+  __device__ __forceinline__ int units() const {
+    const int u = base_units() + slope() * (g.blk + 1);
+    return kUnitSegment + (pair() ? u : u - u / 4);
+  }
+  __device__ __forceinline__ int units_before(int m) const {
+    return (int)((int64_t)m * (kUnitSegment + base_units()) + (int64_t)m * (m + 1) / 2 * slope());
+  }
+  // Tiles of the segment that begin before unit y of it: any rule will do that
+  // only grows with y, from 0 to all of them.
+  __device__ __forceinline__ int tile_at(int y) const {
+    const int u = units();
+    if (y >= u) return g.tiles;
+    if (y <= kUnitSegment) return 0;
+    return (int)__fmul_rn((float)(y - kUnitSegment), __fdiv_rn((float)g.tiles, (float)(u - kUnitSegment)));
+  }
+  // Units of one head of the row space.
+  __device__ __forceinline__ int head_units() {
+    if (g.nblk == 0) return 0;
+    g.blk = g.nblk - 1;
+    return units_before(g.blk) + units();
+  }
+  // To the segment that holds unit y of the row space, `one` units a head; y becomes the unit in the segment.
+  __device__ __forceinline__ void seek(int& y, int one) {
+    g.kh = y / one;
+    y -= g.kh * one;
+    int lo = 0, hi = g.nblk;  // the last block that begins at or before y
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (units_before(mid) <= y)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    g.blk = lo;
+    y -= units_before(lo);
+    size();
   }
   // The next segment of the line.
   __device__ __forceinline__ void next() {
-    if (++g.blk == g.nblk) {
+    if (++g.blk >= g.nblk) {
       g.blk = 0;
-      if (++g.kh == a.hk) {
+      if (++g.kh >= a.hk) {
         g.kh = 0;
         int r = g.req;
         do {
-          if (++r >= a.batch) {  // past the last tile: not walked
-            g.nblk = 0;
-            return;
-          }
+          if (++r >= a.batch) return;  // behind the line's end: not walked
           request(r);
         } while (g.nblk == 0);
       }
@@ -289,38 +359,57 @@ struct Walk {
   }
 };
 
-// What the line holds before request r, prefix first.
-__device__ __forceinline__ int64_t prefix_tiles(const AttnArgs& a, const TilePlan& p, int live) {
-  if (p.joint || a.prefix_len == 0) return 0;
-  return (int64_t)a.hk * (((int64_t)live * a.group + kBlock - 1) / kBlock) * tile_count(a.prefix_len);
+// Units of one head of the prefix's row space.
+__device__ __forceinline__ int prefix_head_units(Walk& w) {
+  if (w.p.joint || w.a.prefix_len == 0) return 0;
+  w.prefix();
+  return w.head_units();
 }
 
-__device__ __forceinline__ int live_tokens(const AttnArgs& a) {
-  const int n = __ldg(a.cu + a.batch);
-  return n < 0 ? 0 : (n > a.tokens ? (int)a.tokens : n);
+// A piece as the other warps get it.
+struct alignas(16) Piece {
+  int n, off, np, own;   // tiles (0: none are left), the first one's number, prefix tiles, own keys of the block
+  int x0, nrow, tok, kh; // rows
+  int req, more, len;    // row x sees own keys below more + x / group + 1 (at most len)
+  int kind;              // 1: the rows' only segment, in one piece; 2: its last piece; 4: the segment in one piece
+  int c0;                // first CTA of the segment
+};
+constexpr int kPieces = 4;
+
+// Keys of tile i of a piece: how many, with `own` own keys in sight; the first one's index among its kind.
+__device__ __forceinline__ int piece_key0(const Piece& g, int i) {
+  const int ti = g.off + i;
+  return (ti < g.np ? ti : ti - g.np) * kKeys;
+}
+__device__ __forceinline__ int piece_keys(const Piece& g, int i, int prefix_len, int own) {
+  const int rest = (g.off + i < g.np ? prefix_len : own) - piece_key0(g, i);
+  return rest < 0 ? 0 : (rest < kKeys ? rest : kKeys);
 }
 
-// Tiles per CTA.
-__device__ __forceinline__ int64_t share(int64_t total, int ctas) { return (total + ctas - 1) / ctas; }
+// Keys of a tile as the products take them: sixteens, at least one.
+__device__ __forceinline__ int sixteens(int keys) { return keys <= 16 ? 1 : (keys + 15) >> 4; }
+
+__device__ __forceinline__ int share(int total, int ctas) {
+  const int n = (total + ctas - 1) / ctas;
+  return n < kMinShare ? kMinShare : n;
+}
 
 // A wait that gives up raises `quit`, which ends every other wait of the CTA.
-__device__ __forceinline__ bool wait_or_quit(uint64_t* bar, uint32_t parity, volatile int* quit) {
-  if (pipe::bar_try(bar, parity)) return true;
-  const uint64_t t0 = pipe::now_ns();
-  while (!pipe::bar_try(bar, parity)) {
-    if (*quit) return false;
-    if (pipe::now_ns() - t0 > pipe::kWaitNs) {
-      *quit = 1;
-      atomicOr(&g_attn_status, 2u);
-      return false;
+// Every lane of the warp gets the same answer.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* quit) {
+  bool ok = pipe::bar_try(bar, parity);
+  if (!__all_sync(0xffffffffu, ok)) {
+    const uint64_t t0 = pipe::now_ns();
+    while (!ok && !(ok = pipe::bar_try(bar, parity))) {
+      if (*quit) break;
+      if (pipe::now_ns() - t0 > pipe::kWaitNs) {
+        *quit = 1;
+        atomicOr(&g_attn_status, 2u);
+        break;
+      }
     }
   }
-  return true;
-}
-
-// The same for a whole warp: every lane gets the same answer.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* quit) {
-  return __all_sync(0xffffffffu, wait_or_quit(bar, parity, quit)) != 0;
+  return __all_sync(0xffffffffu, ok) != 0;
 }
 
 template <int DP>
@@ -333,103 +422,134 @@ struct TileShape {
 
 // Shared memory behind the tiles.
 struct TileShared {
-  float m[2][kRows], l[2][kRows];   // the two warpgroups' halves of the same rows
-  uint64_t full[12], empty[12], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], o_empty, halves, halves_read;
-  alignas(16) int32_t rows[kKeys];  // pool rows of the tile being loaded
-  Segment first;                    // where this CTA's stretch starts
-  int64_t first_off, total;
+  float m[kRows], l[kRows];         // what one warpgroup hands to the other
+  alignas(16) int32_t rows[2][kKeys];  // pool rows of the K and the V tile being loaded
+  uint64_t full[12], empty[12], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], o_empty[2], handed, taken;
+  uint64_t piece_full[kPieces], piece_empty[kPieces];
+  Piece piece[kPieces];
+  Start first;                      // where this CTA's stretch starts
+  int total;
   uint32_t tmem;
   int quit;
 };
 static_assert(sizeof(TileShared) <= 3072, "shared memory behind the tiles");
 
-// Positions in the ring are counted in 32 bits and taken back by a multiple of
-// two turns (which keeps stage and parity) long before they overflow.
-template <int ST>
-constexpr uint32_t kTurn = (1u << 30) / (2 * ST) * (2 * ST);
-template <int ST>
-__device__ __forceinline__ uint32_t next_pos(uint32_t pos, int tiles) {
-  pos += 2 * (uint32_t)tiles;
-  return pos >= kTurn<ST> ? pos - kTurn<ST> : pos;
+// Scores of keys that the row does not see, from `cols` on, become -inf.
+__device__ __forceinline__ void mask_tile(uint32_t ts, int cols) {
+#pragma unroll 1
+  for (int k = 0; k < 128; k += 32) {
+    if (!__any_sync(0xffffffffu, cols < k + 32)) continue;
+    uint32_t x[32];
+    tc::ld32(ts + k, x);
+    tc::wait_ld(x);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) x[e] = k + e < cols ? x[e] : 0xff800000u;
+    tc::st32(ts + k, x);
+  }
+  tc::wait_st();
+}
+
+__device__ __forceinline__ float max32(const uint32_t* x, float m) {
+  float t[2] = {m, m};
+#pragma unroll
+  for (int e = 0; e < 32; e += 4) {
+    t[0] = fmaxf(fmaxf(t[0], __uint_as_float(x[e])), __uint_as_float(x[e + 1]));
+    t[1] = fmaxf(fmaxf(t[1], __uint_as_float(x[e + 2])), __uint_as_float(x[e + 3]));
+  }
+  return fmaxf(t[0], t[1]);
+}
+
+// 32 scores become 16 words of P; returns their sum.
+template <typename T>
+__device__ __forceinline__ float exp32(uint32_t* x, float c, float mc) {
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int e = 0; e < 32; e += 2) {
+    const float p0 = tc::ex2(fmaf(__uint_as_float(x[e]), c, -mc)), p1 = tc::ex2(fmaf(__uint_as_float(x[e + 1]), c, -mc));
+    sum[(e >> 1) & 3] += p0 + p1;
+    x[e >> 1] = Vec16<T>::pack2(p0, p1);
+  }
+  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
 // One row's share of a tile: the scores at tensor memory `ts` (128 columns) become
 // 16-bit P there; (m, l) follow, and O at `to` (when it holds something) is
-// brought to the new reference. CUT: only the first `cols` keys are seen.
-template <typename T, int DP, bool CUT>
-__device__ __forceinline__ void softmax_tile(uint32_t ts, uint32_t to, float c, int cols, bool has_o, float& m,
-                                             float& l) {
-  uint32_t s[128];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) tc::ld32(ts + k * 32, s + k * 32);
-  tc::wait_ld();
-  float t4[4] = {m, m, m, m};
-#pragma unroll
-  for (int k = 0; k < 128; ++k)
-    if (!CUT || k < cols) t4[k & 3] = fmaxf(t4[k & 3], __uint_as_float(s[k]));
-  const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+// brought to the new reference. What a lane without a row (!on) computes is not
+// read. The scores are read twice, 64 columns at a time: that costs less than
+// the registers and the code of 128 at once.
+template <typename T, int DP>
+__device__ __forceinline__ void softmax_tile(uint32_t ts, uint32_t to, float c, bool on, bool has_o, float& m, float& l) {
+  uint32_t x[32], y[32];
+  float top = m;
+#pragma unroll 1
+  for (int k = 0; k < 128; k += 64) {
+    tc::ld32(ts + k, x);
+    tc::ld32(ts + k + 32, y);
+    tc::wait_ld(x);
+    tc::wait_ld(y);
+    top = max32(y, max32(x, top));
+  }
   // move the reference when it is too far behind (or there is none yet)
-  const bool move = (top - m) * c > 8.f || (m == -INFINITY && top > -INFINITY);
+  const bool move = on && ((top - m) * c > 8.f || (m == -INFINITY && top > -INFINITY));
   if (__any_sync(0xffffffffu, move)) {
     const float f = !move ? 1.f : (m == -INFINITY ? 0.f : tc::ex2((m - top) * c));
     if (move) m = top;
     l *= f;
     if (has_o) {
-      uint32_t o[32];
 #pragma unroll 1
       for (int k = 0; k < DP; k += 32) {
-        tc::ld32(to + k, o);
-        tc::wait_ld();
+        tc::ld32(to + k, x);
+        tc::wait_ld(x);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-        tc::st32(to + k, o);
+        for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+        tc::st32(to + k, x);
       }
     }
   }
   const float mc = m == -INFINITY ? 0.f : m * c;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int k = h * 64; k < h * 64 + 64; k += 2) {
-      float p0 = tc::ex2(fmaf(__uint_as_float(s[k]), c, -mc));
-      float p1 = tc::ex2(fmaf(__uint_as_float(s[k + 1]), c, -mc));
-      if (CUT) {
-        p0 = k < cols ? p0 : 0.f;
-        p1 = k + 1 < cols ? p1 : 0.f;
-      }
-      sum[(k >> 1) & 3] += p0 + p1;
-      s[k >> 1] = Vec16<T>::pack2(p0, p1);
-    }
-    tc::st32(ts + h * 32, s + h * 32);
+  // P's words overlay the scores from the left: 32 columns of scores are read before the 16 words go out
+  tc::ld32(ts, x);
+#pragma unroll 1
+  for (int k = 0; k < 128; k += 64) {
+    tc::wait_ld(x);
+    tc::ld32(ts + k + 32, y);
+    l += exp32<T>(x, c, mc);
+    tc::wait_ld(y);
+    tc::st16(ts + k / 2, x);
+    if (k == 0) tc::ld32(ts + 64, x);
+    l += exp32<T>(y, c, mc);
+    tc::st16(ts + k / 2 + 16, y);
   }
-  l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  tc::wait_st();
 }
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const AttnArgs a, const TilePlan p,
                                                                      const __grid_constant__ PoolMaps maps) {
   using Shape = TileShape<DP>;
-  constexpr int ST = Shape::stages;
-  constexpr bool kBf16 = Vec16<T>::bf16;
+  constexpr uint32_t ST = Shape::stages;
   extern __shared__ __align__(1024) unsigned char smem[];
   TileShared& sh = *reinterpret_cast<TileShared*>(smem + Shape::data);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int i = 0; i < ST; ++i) {
+    for (int i = 0; i < (int)ST; ++i) {
       pipe::bar_init(sh.full + i, 1);
       pipe::bar_init(sh.empty + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
-      pipe::bar_init(sh.q_full + i, 2);
+      pipe::bar_init(sh.q_full + i, 1);
       pipe::bar_init(sh.q_empty + i, 1);
       pipe::bar_init(sh.s_full + i, 1);
       pipe::bar_init(sh.p_full + i, 4);
       pipe::bar_init(sh.o_full + i, 1);
+      pipe::bar_init(sh.o_empty + i, 4);
     }
-    pipe::bar_init(&sh.o_empty, 8);
-    pipe::bar_init(&sh.halves, 8);
-    pipe::bar_init(&sh.halves_read, 8);
+    for (int i = 0; i < kPieces; ++i) {
+      pipe::bar_init(sh.piece_full + i, 1);
+      pipe::bar_init(sh.piece_empty + i, 12);  // 8 softmax warps, both loads, scores and sums of the products
+    }
+    pipe::bar_init(&sh.handed, 4);
+    pipe::bar_init(&sh.taken, 4);
     pipe::bar_init_fence();
     sh.quit = (tc::smem_addr(smem) & 1023u) != 0;  // the swizzle counts from 1024-byte patterns
     if (sh.quit) atomicOr(&g_attn_status, 2u);
@@ -438,124 +558,125 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
     tc::alloc(&sh.tmem, 512);
     tc::relinquish();
   }
+  if (warp == 9 && lane < 2) {
+    tc::prefetch_map(maps.box + lane);
+    tc::prefetch_map(maps.row + lane);
+  }
   grid_dep_wait();
   grid_dep_launch();
 
-  // The line: tiles of every request (a run of requests per thread), their sum,
+  // The line: units of every request (a run of requests per thread), their sums,
   // and the place where this CTA's stretch starts.
   const int live = live_tokens(a);
   {
     Walk w(a, p, live);
-    int64_t* wsum = reinterpret_cast<int64_t*>(smem);  // the tiles' memory is not in use yet
+    int* wsum = reinterpret_cast<int*>(smem);  // the tiles' memory is not in use yet
     const int per = (a.batch + kTileThreads - 1) / kTileThreads;
     const int r0 = tid * per < a.batch ? tid * per : a.batch, r1 = r0 + per < a.batch ? r0 + per : a.batch;
-    int64_t mine = 0, last = 0;  // tiles of the run, of one head of its last request
+    int mine = 0, one = 0;  // units of the run, of one head of its last request
     for (int r = r0; r < r1; ++r) {
       w.request(r);
-      last = w.head_tiles();
-      mine += last * a.hk;
-      if (blockIdx.x == 0 && (__ldg(a.lens + r) > (int64_t)a.width * a.page || __ldg(a.lens + r) < 0 ||
-                              __ldg(a.cu + r) < 0 || __ldg(a.cu + r + 1) > a.tokens ||
-                              __ldg(a.cu + r + 1) < __ldg(a.cu + r)))
-        atomicOr(&g_attn_status, 1u);
+      one = w.head_units();
+      mine += one * a.hk;
+      if (blockIdx.x == 0 && !w.fits(r)) atomicOr(&g_attn_status, 1u);
     }
-    int64_t x = mine;
+    int x = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+      const int y = __shfl_up_sync(0xffffffffu, x, d);
       if (lane >= d) x += y;
     }
     if (lane == 31) wsum[warp] = x;
+    const int pre_one = prefix_head_units(w), pre = pre_one * a.hk;
     __syncthreads();
-    const int64_t pre = prefix_tiles(a, p, live);
-    int64_t at = pre + x - mine, total = pre;
+    int at = pre + x - mine, total = pre;
+#pragma unroll
     for (int i = 0; i < kTileThreads / 32; ++i) {
-      if (i < warp) at += wsum[i];
-      total += wsum[i];
+      const int v = wsum[i];
+      if (i < warp) at += v;
+      total += v;
     }
-    const int64_t x0 = (int64_t)blockIdx.x * share(total, p.ctas);
+    const int x0 = (int)blockIdx.x * share(total, p.ctas);
     if (tid == 0) {
       sh.total = total;
       if (x0 < pre) {
-        w.prefix_space();
-        const int tp = tile_count(a.prefix_len);
-        const int64_t si = x0 / tp;
-        w.g.kh = (int)(si / w.g.nblk);
-        w.g.blk = (int)(si - (int64_t)w.g.kh * w.g.nblk);
-        w.g.tiles = tp;
-        sh.first = w.g;
-        sh.first_off = x0 - si * tp;
+        w.prefix();
+        sh.first.y = x0;
+        w.seek(sh.first.y, pre_one);
+        sh.first.g = w.g;
       }
     }
     for (int r = r0; r < r1; ++r) {
       if (per > 1) {
         w.request(r);
-        last = w.head_tiles();
+        one = w.head_units();
       }
-      const int64_t one = last;
-      if (blockIdx.x == 0) p.start[r] = at;
       if (x0 >= at && x0 < at + one * a.hk) {
-        int64_t y = x0 - at;
-        w.g.kh = (int)(y / one);
-        y -= w.g.kh * one;
-        for (w.g.blk = 0;; ++w.g.blk) {
-          w.size();
-          if (y < w.g.tiles) break;
-          y -= w.g.tiles;
-        }
-        sh.first = w.g;
-        sh.first_off = y;
+        w.request(r);
+        int y = x0 - at;
+        w.seek(y, one);
+        sh.first.y = y;
+        sh.first.g = w.g;
       }
       at += one * a.hk;
     }
-    if (blockIdx.x == 0 && tid == 0) p.start[a.batch] = total;
+    if (tid < 2) p.used[2 * blockIdx.x + tid] = 0;
+    if (tid == 2) p.end[blockIdx.x].nrow = 0;
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
   }
   const uint32_t tmem = sh.tmem;
-  const int64_t unit = share(sh.total, p.ctas);
-  const int64_t x0 = (int64_t)blockIdx.x * unit, x1 = x0 + unit < sh.total ? x0 + unit : sh.total;
+  const int unit = share(sh.total, p.ctas);
+  const int x0 = (int)blockIdx.x * unit, x1 = sh.total - x0 < unit ? sh.total : x0 + unit;
   volatile int* quit = &sh.quit;
   const float c = fabsf(a.scale) * 1.4426950408889634f;
-
   if (x0 < x1 && !*quit) {
-    Walk w(a, p, live);
-    w.g = sh.first;
-    int64_t left = x1 - x0;
-    int off = (int)sh.first_off;
+    // Reads piece number `i` of the CTA; whoever has read it says so with done_piece.
+    const auto next_piece = [&](uint32_t i) { return warp_wait(sh.piece_full + i % kPieces, (i / kPieces) & 1, quit); };
+    const auto done_piece = [&](uint32_t i) {
+      __syncwarp();
+      if (lane == 0) pipe::bar_arrive(sh.piece_empty + i % kPieces);
+    };
+    const uint32_t base = tc::smem_addr(smem), ring = base + 2 * Shape::tile;
     if (warp < 8) {
       // ------------------------------------------------ softmax warpgroups ----
-      tc::regs_up<kSoftmaxRegs>();
       const int t = warp >> 2, r = tid & (kRows - 1);
       const uint32_t row = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t ts = tmem + row + t * 128, to = tmem + row + 256 + t * 128;
-      uint32_t n_s = 0, n_piece = 0, n_halves = 0, n_o[2] = {0, 0};
-      while (true) {
-        const int rows = w.rows(), n = (int)(w.g.tiles - off < left ? w.g.tiles - off : left);
-        const bool pair = rows > kRows;
-        const int mine = pair ? t * kRows + r : r;             // this thread's row of the block
-        const int np = w.prefix_part();
-        const int64_t see = mine < rows ? w.row_seen(w.g.blk * kBlock + mine) : 0;
-        const bool warp_on = __any_sync(0xffffffffu, mine < rows);
+      uint32_t n_s = 0, n_handed = 0, n_o[2] = {0, 0}, step = 0;
+      for (uint32_t pi = 0;; ++pi) {
+        if (!next_piece(pi)) break;
+        const Piece& g = sh.piece[pi % kPieces];
+        const int n = g.n;
+        if (n == 0) break;
+        const int u0 = step & 1, half = t ^ u0;                 // half of the block, or first tile
+        const bool two = g.nrow > kRows, shared = !two && n > 1;  // shared: both warpgroups hold tiles of the rows
+        step += two ? 2 * n : n;
+        const uint32_t turn = n_o[t], turn_other = n_o[t ^ 1];
+        n_o[u0] += 1;
+        n_o[u0 ^ 1] += two || shared;
+        if (!two && !shared && half) {
+          done_piece(pi);
+          continue;
+        }
+        const int brow = (two ? half * kRows : 0) + r, x = g.x0 + brow;  // this thread's row: of the block, of the row space
+        const bool on = brow < g.nrow;
+        const bool warp_on = __any_sync(0xffffffffu, on);
+        const int jt = (int)a.group_div.div((uint32_t)x);
+        int see = g.more + jt + 1;
+        see = see < 0 ? 0 : (see > g.len ? g.len : see);
         float m = -INFINITY, l = 0.f;
         bool ok = true;
-        for (int i = pair ? 0 : t; i < n; i += pair ? 1 : 2) {
-          ok = warp_wait(sh.s_full + t, n_s & 1, quit);
-          if (!ok) break;
+#pragma unroll 1
+        for (int i = two ? 0 : half; i < n; i += two ? 1 : 2) {
+          if (!(ok = warp_wait(sh.s_full + t, n_s & 1, quit))) break;
           ++n_s;
           tc::fence_after();
           if (warp_on) {
-            const int ti = off + i;
-            const int64_t rest = ti >= np ? see - (int64_t)(ti - np) * kKeys
-                                          : (mine < rows ? a.prefix_len - ti * kKeys : 0);
-            const int cols = rest < 0 ? 0 : (rest < kKeys ? (int)rest : kKeys);
-            const bool has_o = pair ? i > 0 : i >= 2;
-            if (__any_sync(0xffffffffu, cols < kKeys))
-              softmax_tile<T, DP, true>(ts, to, c, cols, has_o, m, l);
-            else
-              softmax_tile<T, DP, false>(ts, to, c, cols, has_o, m, l);
-            tc::wait_st();
+            const int cols = on ? piece_keys(g, i, a.prefix_len, see) : kKeys;
+            if (__any_sync(0xffffffffu, cols < kKeys)) mask_tile(ts, cols);
+            softmax_tile<T, DP>(ts, to, c, on, two ? i > 0 : i >= 2, m, l);
           }
           tc::fence_before();
           __syncwarp();
@@ -563,301 +684,348 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
         }
         if (!ok) break;
         // -------------------------------------------------------- results ----
-        // the product of the last tile; in single blocks both halves' products
-        const bool has[2] = {true, pair || n > 1};
-        for (int u = 0; u < 2; ++u) {
-          if (has[u] && (!pair || u == t)) ok = ok && warp_wait(sh.o_full + u, n_o[u] & 1, quit);
-          n_o[u] += has[u];
-        }
-        if (!ok) break;
-        tc::fence_after();
+        // The warpgroup that has the last tile takes over the other's maximum and
+        // sum; it can read both results in tensor memory.
         float w0 = 1.f, w1 = 0.f;
-        if (!pair && n > 1) {
-          if (n_halves > 0 && !(ok = warp_wait(&sh.halves_read, (n_halves - 1) & 1, quit))) break;
-          sh.m[t][r] = m;
-          sh.l[t][r] = l;
-          __syncwarp();
-          if (lane == 0) pipe::bar_arrive(&sh.halves);
-          if (!(ok = warp_wait(&sh.halves, n_halves & 1, quit))) break;
-          const float ma = sh.m[0][r], mb = sh.m[1][r], la = sh.l[0][r], lb = sh.l[1][r];
-          __syncwarp();
-          if (lane == 0) pipe::bar_arrive(&sh.halves_read);
-          ++n_halves;
-          m = fmaxf(ma, mb);
-          w0 = ma == -INFINITY ? 0.f : tc::ex2((ma - m) * c);
-          w1 = mb == -INFINITY ? 0.f : tc::ex2((mb - m) * c);
-          // a sum that is not a number stays so, whatever its maximum
-          l = (la == la ? w0 * la : la) + (lb == lb ? w1 * lb : lb);
-        }
-        const bool whole = off == 0 && n == w.g.tiles;
-        const bool direct = whole && (p.joint || a.prefix_len == 0);
-        const bool split_cols = !pair && n > 1;                 // both warpgroups write half the columns
-        const bool writes = mine < rows && (pair || n > 1 || t == 0);
-        const int x = w.g.blk * kBlock + mine;
-        const int jt = (int)a.group_div.div((uint32_t)x);
-        const int64_t grow = ((int64_t)w.g.tok + jt) * a.hq + w.g.kh * a.group + (x - jt * a.group);
-        const int64_t crow = ((int64_t)2 * blockIdx.x + (off == 0 ? 1 : 0)) * kBlock + mine;
-        const int64_t wrow = (w.g.req < 0 ? 0 : (int64_t)a.tokens * a.hq) + grow;
-        float* dst = whole ? p.whole + wrow * a.dim : p.cut + crow * a.dim;
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        const float ls = l == 0.f ? -INFINITY : m * c + log2f(l);
-        if (writes && (t == 0 || pair)) {
-          if (direct) {
-            if (a.lse) a.lse[grow] = ls * 0.6931471805599453f;
-          } else {
-            (whole ? p.whole_lse[wrow] : p.cut_lse[crow]) = ls;
+        if (shared) {
+          const uint32_t turn_h = n_handed++;
+          if (half != ((n - 1) & 1)) {
+            if (turn_h > 0 && !warp_wait(&sh.taken, (turn_h - 1) & 1, quit)) break;
+            sh.m[r] = m;
+            sh.l[r] = l;
+            __syncwarp();
+            if (lane == 0) pipe::bar_arrive(&sh.handed);
+            done_piece(pi);
+            continue;
           }
+          if (!warp_wait(&sh.handed, turn_h & 1, quit)) break;
+          const float mb = sh.m[r], lb = sh.l[r];
+          __syncwarp();
+          if (lane == 0) pipe::bar_arrive(&sh.taken);
+          const float top = fmaxf(m, mb);
+          w0 = m == -INFINITY ? 0.f : tc::ex2((m - top) * c);
+          w1 = mb == -INFINITY ? 0.f : tc::ex2((mb - top) * c);
+          // a sum that is not a number stays so, whatever its maximum
+          l = (l == l ? w0 * l : l) + (lb == lb ? w1 * lb : lb);
+          m = top;
+          if (!warp_wait(sh.o_full + (t ^ 1), turn_other & 1, quit)) break;
         }
-        if (warp_on && (pair || n > 1 || t == 0)) {
-          const int k0 = split_cols ? t * (DP / 2) : 0, k1 = split_cols ? k0 + DP / 2 : DP;
-          const uint32_t oa = pair ? to : tmem + row + 256, ob = tmem + row + 384;
-#pragma unroll 1
-          for (int k = k0; k < k1; k += 32) {
-            if (k >= a.dim) break;
-            uint32_t o[32], o2[32];
-            tc::ld32(oa + k, o);
-            if (split_cols) tc::ld32(ob + k, o2);
-            tc::wait_ld();
-            float f[32];
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              f[e] = __uint_as_float(o[e]);
-              if (split_cols) f[e] = f[e] * w0 + __uint_as_float(o2[e]) * w1;
-              f[e] = l == 0.f ? 0.f : f[e] * inv;
+        if (!warp_wait(sh.o_full + t, turn & 1, quit)) break;
+        tc::fence_after();
+        if (warp_on) {
+          const bool direct = g.kind & 1, whole = g.kind & 4;
+          const int u = g.req < 0 ? 0 : 1;
+          const int64_t all = a.tokens * a.hq;
+          const int64_t grow = ((int64_t)g.tok + jt) * a.hq + g.kh * a.group + (x - jt * a.group);
+          const int slot = 2 * blockIdx.x + (g.off == 0 ? 1 : 0);
+          const int64_t part = whole ? u * all + grow : (int64_t)slot * kBlock + brow;
+          float* dst = (whole ? p.whole : p.cut) + part * a.dim;
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          if (on) {
+            const float ls = l == 0.f ? -INFINITY : m * c + log2f(l);
+            if (direct) {
+              if (a.lse) a.lse[grow] = ls * 0.6931471805599453f;
+            } else {
+              (whole ? p.whole_lse : p.cut_lse)[part] = ls;
+              if (!whole && brow == 0) p.used[slot] = 1;
+              if ((g.kind & 2) && !p.joint)
+                p.place[u * all + grow] = whole ? make_int2(-1, -1) : make_int2(g.c0 | brow << 16, blockIdx.x);
+              if ((g.kind & 2) && p.joint && brow == 0)
+                p.end[blockIdx.x] = CutEnd{g.nrow, g.c0, g.tok, g.kh, g.x0};
             }
-            if (writes) {
-              if (direct) {
-                char* to_row = a.out + (grow * a.dim + k) * 2;
+          }
+          w0 *= inv;
+          w1 *= inv;
+#pragma unroll 1
+          for (int k = 0; k < a.dim; k += 32) {
+            uint32_t o[32], o2[32];
+            tc::ld32(to + k, o);
+            if (shared) tc::ld32(tmem + row + 256 + (t ^ 1) * 128 + k, o2);
+            tc::wait_ld(o);
+            if (shared) {
+              tc::wait_ld(o2);
 #pragma unroll
-                for (int e = 0; e < 32; e += 8)
-                  if (k + e < a.dim) *reinterpret_cast<uint4*>(to_row + e * 2) = Vec16<T>::pack(f + e);
-              } else {
+              for (int e = 0; e < 32; ++e)
+                o[e] = __float_as_uint(__uint_as_float(o[e]) * w0 + __uint_as_float(o2[e]) * w1);
+            } else {
 #pragma unroll
-                for (int e = 0; e < 32; e += 4)
-                  if (k + e < a.dim)
-                    *reinterpret_cast<float4*>(dst + k + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
-              }
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * w0);
+            }
+            if (l == 0.f) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = 0u;
+            }
+            if (!on) continue;
+            if (direct) {
+              char* to_row = a.out + (grow * a.dim + k) * 2;
+#pragma unroll
+              for (int e = 0; e < 32; e += 8)
+                if (k + e < a.dim)
+                  *reinterpret_cast<uint4*>(to_row + e * 2) = Vec16<T>::pack(reinterpret_cast<const float*>(o) + e);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; e += 4)
+                if (k + e < a.dim) *reinterpret_cast<uint4*>(dst + k + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
           }
         }
         tc::fence_before();
         __syncwarp();
-        if (lane == 0) pipe::bar_arrive(&sh.o_empty);
-        ++n_piece;
-        left -= n;
-        if (left <= 0) break;
-        off = 0;
-        w.next();
+        if (lane == 0) {
+          pipe::bar_arrive(sh.o_empty + t);
+          if (shared) pipe::bar_arrive(sh.o_empty + (t ^ 1));
+        }
+        done_piece(pi);
       }
-    } else {
-    tc::regs_down<kOtherRegs>();
-    if (warp == 8) {
+    } else if (warp == 8) {
       // -------------------------------------------------------- products ----
-      // The whole warp walks along; one lane issues.
-      const uint32_t id_s = tc::idesc(kBf16, kRows, kKeys, false, a.scale < 0.f);
-      const uint32_t id_o = tc::idesc(kBf16, kRows, a.dim, true);
+      // The whole warp walks along; one lane issues. Step s runs on S, P and O
+      // number s & 1; its scores are issued right after the P V of step s - 2.
+      const uint32_t id_s = tc::idesc(Vec16<T>::bf16, kRows, 0, false, a.scale < 0.f);
+      const uint32_t id_o = tc::idesc(Vec16<T>::bf16, kRows, a.dim, true);
       const int ks = a.dim / 16;
-      const uint32_t base = tc::smem_addr(smem), ring = base + 2 * Shape::tile;
-      uint32_t n_p[2] = {0, 0}, n_piece = 0, n_q = 0;
-      uint32_t pos = 0;  // counts K and V tiles, modulo 2^32 in whole turns of the ring
-      bool ok = true;
-      while (ok) {
-        const int rows = w.rows(), n = (int)(w.g.tiles - off < left ? w.g.tiles - off : left);
-        const bool pair = rows > kRows;
-        const int nq = pair ? 2 : 1;
-        for (int b = 0; b < nq && ok; ++b)
-          ok = warp_wait(sh.q_full + ((n_q + b) & 1), ((n_q + b) >> 1) & 1, quit);
-        if (!ok) break;
-        const uint32_t q0 = base + (n_q & 1) * Shape::tile, q1 = pair ? base + ((n_q + 1) & 1) * Shape::tile : q0;
-        const auto tile_of = [&](int k, int t) { return pair ? k : 2 * k + t; };
-        const auto scores = [&](int k, int t) {
-          const int i = tile_of(k, t);
-          if (i >= n) return true;
-          const uint32_t at = pos + 2 * (uint32_t)i, st = at % ST;
-          if (!warp_wait(sh.full + st, (at / ST) & 1, quit)) return false;
-          tc::fence_after();
-          const uint64_t qd = tc::desc(t ? q1 : q0, 16, 1024), kd = tc::desc(ring + st * Shape::tile, 16, 1024);
-          if (tc::elect()) {
-#pragma unroll
-            for (int j = 0; j < DP / 16; ++j) {
-              const uint32_t o = ((j >> 2) * (kRows * 128) + (j & 3) * 32) >> 4;
-              if (j < ks) tc::mma_ss(tmem + t * 128, qd + o, kd + o, id_s, j > 0);
-            }
-            tc::commit(sh.s_full + t);
-            if (!pair || t == 1) tc::commit(sh.empty + st);
+      uint32_t n_p[2] = {0, 0}, n_o[2] = {0, 0}, n_q = 0;
+      // the scores' place: piece, tile, step of the tile; the sums' place
+      uint32_t qp = 0, qs = 0, qt = 0, wp = 0, wt = 0;
+      int qi = 0, qsub = 0, qn = 0, wn = 0;
+      bool qtwo = false, more = true;
+      const auto scores = [&]() {
+        if (!more) return true;
+        if (qi == 0 && qsub == 0) {
+          if (!next_piece(qp)) return false;
+          qn = sh.piece[qp % kPieces].n;
+          qtwo = sh.piece[qp % kPieces].nrow > kRows;
+          if (qn == 0) {
+            more = false;
+            return true;
           }
-          __syncwarp();
-          return true;
-        };
-        ok = scores(0, 0) && scores(0, 1);
-        for (int k = 0; ok && tile_of(k, 0) < n; ++k) {
-          for (int t = 0; ok && t < 2; ++t) {
-            const int i = tile_of(k, t);
-            if (i >= n) break;
-            const uint32_t at = pos + 2 * (uint32_t)i + 1, st = at % ST;
-            ok = warp_wait(sh.full + st, (at / ST) & 1, quit) && warp_wait(sh.p_full + t, n_p[t] & 1, quit);
-            if (!ok) break;
-            ++n_p[t];
-            if (k == 0 && t == 0 && n_piece > 0 && !(ok = warp_wait(&sh.o_empty, (n_piece - 1) & 1, quit))) break;
+        }
+        const int l2 = qs & 1;
+        if (qi == 0 && !warp_wait(sh.q_full + ((n_q + qsub) & 1), ((n_q + qsub) >> 1) & 1, quit)) return false;
+        const uint32_t at = 2 * qt, st = at % ST;
+        if (!warp_wait(sh.full + st, (at / ST) & 1, quit)) return false;
+        tc::fence_after();
+        const Piece& g = sh.piece[qp % kPieces];
+        const uint32_t id = id_s | (uint32_t)(2 * sixteens(piece_keys(g, qi, a.prefix_len, g.own))) << 17;
+        const uint64_t qd = tc::desc(base + ((n_q + qsub) & 1) * Shape::tile, 16, 1024);
+        const uint64_t kd = tc::desc(ring + st * Shape::tile, 16, 1024);
+        const bool tile_done = !qtwo || qsub == 1, done = tile_done && qi == qn - 1;
+        if (tc::elect()) {
+#pragma unroll
+          for (int j = 0; j < DP / 16; ++j) {
+            const uint32_t o = ((j >> 2) * (kRows * 128) + (j & 3) * 32) >> 4;
+            if (j < ks) tc::mma_ss(tmem + l2 * 128, qd + o, kd + o, id, j > 0);
+          }
+          tc::commit(sh.s_full + l2);
+          if (tile_done) tc::commit(sh.empty + st);
+          if (done) {
+            tc::commit(sh.q_empty + (n_q & 1));
+            if (qtwo) tc::commit(sh.q_empty + ((n_q + 1) & 1));
+          }
+        }
+        __syncwarp();
+        ++qs;
+        qsub = tile_done ? 0 : 1;
+        if (tile_done) {
+          ++qt;
+          ++qi;
+        }
+        if (done) {
+          n_q += qtwo ? 2 : 1;
+          qi = 0;
+          done_piece(qp++);
+        }
+        return true;
+      };
+      bool ok = scores() && scores();
+      for (uint32_t s = 0; ok; ++wp) {
+        if (!next_piece(wp)) break;
+        const Piece& g = sh.piece[wp % kPieces];
+        wn = g.n;
+        const bool two = g.nrow > kRows;
+        if (wn == 0) break;
+#pragma unroll 1
+        for (int i = 0; ok && i < wn; ++i, ++wt) {
+          const uint32_t at = 2 * wt + 1, st = at % ST;
+          const int kk = sixteens(piece_keys(g, i, a.prefix_len, g.own));
+          const bool fresh = two ? i == 0 : i < 2, last = two ? i == wn - 1 : i >= wn - 2;
+          if (!(ok = warp_wait(sh.full + st, (at / ST) & 1, quit))) break;
+#pragma unroll 1
+          for (int sub = 0; sub <= (two ? 1 : 0); ++sub, ++s) {
+            const int l2 = s & 1;
+            if (!(ok = warp_wait(sh.p_full + l2, n_p[l2] & 1, quit))) break;
+            ++n_p[l2];
+            if (fresh) {
+              if (n_o[l2] > 0 && !(ok = warp_wait(sh.o_empty + l2, (n_o[l2] - 1) & 1, quit))) break;
+              ++n_o[l2];
+            }
             tc::fence_after();
             const uint64_t vd = tc::desc(ring + st * Shape::tile, kKeys * 128, 1024);
             if (tc::elect()) {
 #pragma unroll
               for (int j = 0; j < kKeys / 16; ++j)
-                tc::mma_ts(tmem + 256 + t * 128, tmem + t * 128 + j * 8, vd + ((j * 2048) >> 4), id_o, k > 0 || j > 0);
-              if (!pair || t == 1) tc::commit(sh.empty + st);
-              if (tile_of(k + 1, t) >= n) tc::commit(sh.o_full + t);
+                if (j < kk)
+                  tc::mma_ts(tmem + 256 + l2 * 128, tmem + l2 * 128 + j * 8, vd + ((j * 2048) >> 4), id_o, !fresh || j > 0);
+              if (!two || sub == 1) tc::commit(sh.empty + st);
+              if (last) tc::commit(sh.o_full + l2);
             }
             __syncwarp();
-            ok = scores(k + 1, t);
+            if (!(ok = scores())) break;
           }
+        }
+        done_piece(wp);
+      }
+    } else if (warp < 11) {
+      // --------------------------------------------------- loads of K, V ----
+      // Whole pages as boxes; the rest of a tile, or a tile with a page outside
+      // the pool, four rows at a time, with zeros for what is not there (a slot
+      // behind the end may hold anything). Only the sixteens that the products
+      // take are loaded.
+      constexpr int PN = DP / 64;                               // 64-value panels of a row
+      constexpr uint32_t kPanel = kRows * 128;
+      const int kv = warp - 9, none = (int)a.pool_rows;         // none: a row outside the map
+      const CUtensorMap *box = maps.box + kv, *one_row = maps.row + kv;
+      int32_t* rows = sh.rows[kv];
+      uint32_t pos = kv;
+      bool ok = true;
+      for (uint32_t pi = 0; ok; ++pi) {
+        if (!next_piece(pi)) break;
+        const Piece& g = sh.piece[pi % kPieces];
+        const int n = g.n, x = g.kh * a.dim;
+        if (n == 0) break;
+#pragma unroll 1
+        for (int i = 0; i < n; ++i, pos += 2) {
+          const int k0 = piece_key0(g, i) + (g.off + i < g.np ? 0 : a.prefix_len), valid = piece_keys(g, i, a.prefix_len, g.own);
+          int boxes = p.run > 0 ? valid / p.run : 0;
+          int32_t y = 0;
+          if (lane < boxes) {
+            const int64_t sl = key_slot(a, g.req, k0 + lane * p.run);
+            y = sl < 0 || sl + p.run > a.pool_rows ? -1 : (int32_t)sl;
+          }
+          if (__any_sync(0xffffffffu, y < 0)) boxes = 0;
+          if (lane < boxes) rows[lane] = y;
+          const int quad0 = boxes * p.run / 4, quads = sixteens(valid) * 4;
+          if (lane >= quad0 && lane < quads) {
+            int32_t* z = rows + lane * 4;                       // behind the boxes' entries
+#pragma unroll 1
+            for (int j = 0; j < 4; ++j) {
+              z[j] = none;
+              if (lane * 4 + j < valid) {
+                const int64_t sl = key_slot(a, g.req, k0 + lane * 4 + j);
+                if (sl >= 0) z[j] = (int32_t)sl;
+              }
+            }
+          }
+          const uint32_t st = pos % ST;
+          __syncwarp();
+          if (pos >= ST && !(ok = warp_wait(sh.empty + st, (pos / ST - 1) & 1, quit))) break;
+          if (tc::elect()) {
+            uint32_t dst = ring + st * Shape::tile;
+            pipe::bar_expect_tx(sh.full + st, (uint32_t)quads * 4 * DP * 2);
+#pragma unroll 1
+            for (int b = 0; b < boxes; ++b, dst += p.run * 128) {
+              const int yb = rows[b];
+#pragma unroll
+              for (int pn = 0; pn < PN; ++pn) tc::load_box(dst + pn * kPanel, box, x + pn * 64, yb, sh.full + st);
+            }
+#pragma unroll 1
+            for (int b = quad0; b < quads; ++b, dst += 512) {
+              const int4 z = *reinterpret_cast<const int4*>(rows + b * 4);
+#pragma unroll
+              for (int pn = 0; pn < PN; ++pn) tc::load_rows(dst + pn * kPanel, one_row, x + pn * 64, z, sh.full + st);
+            }
+          }
+          __syncwarp();
+        }
+        done_piece(pi);
+      }
+      // copies must not outlive the CTA: all are waited for by the products, unless a wait gave up
+      if (*quit)
+        for (uint32_t q = kv; q < pos; q += 2)
+          if (q + 2 * ST >= pos) (void)pipe::bar_wait(sh.full + q % ST, (q / ST) & 1);
+    } else {
+      // ------------------------------------------ the walk, loads of Q ----
+      constexpr int CH = DP / 8, RI = 32 / CH;                  // 16-byte chunks of a row; rows per instruction
+      const int ch = lane % CH, sub = lane / CH;
+      const bool in_dim = ch * 8 < a.dim;
+      const uint32_t panel = (uint32_t)(ch >> 3) * (kRows * 128);
+      Walk w(a, p, live);
+      w.g = sh.first.g;
+      int y = sh.first.y, left = x1 - x0, at = x0 - y;          // units into the segment, left of the stretch; its start
+      uint32_t n_q = 0, pi = 0;
+      bool ok = true;
+#pragma unroll 1
+      while (true) {
+        const int units = left > 0 ? w.units() : 0;
+        const int off = left > 0 ? w.tile_at(y) : 0, end = left > 0 ? w.tile_at(left < units - y ? y + left : units) : 0;
+        if (left > 0 && end == off) {                           // no tile of the segment begins here
+          left -= units - y;
+          at += units;
+          y = 0;
+          if (left > 0) w.next();
+          continue;
+        }
+        const int slot = pi % kPieces, nrow = w.rows();
+        if (pi >= kPieces && !(ok = warp_wait(sh.piece_empty + slot, (pi / kPieces - 1) & 1, quit))) break;
+        if (lane == 0) {
+          Piece& g = sh.piece[slot];
+          g.n = end - off;
+          if (left > 0) {
+            const bool whole = end - off == w.g.tiles;
+            g.off = off;
+            g.np = w.prefix_part();
+            g.own = w.own_keys();
+            g.x0 = w.g.blk * kBlock;
+            g.nrow = nrow;
+            g.tok = w.g.tok;
+            g.kh = w.g.kh;
+            g.req = w.g.req;
+            g.more = w.g.len - w.g.ntok;
+            g.len = w.g.len;
+            g.kind = (whole && p.joint ? 1 : 0) | (end == w.g.tiles ? 2 : 0) | (whole ? 4 : 0);
+            int c0 = at / unit;                                 // the stretch in which its first tile begins
+            while (c0 < (int)blockIdx.x && w.tile_at((c0 + 1) * unit - at) == 0) ++c0;
+            g.c0 = c0;
+          }
+        }
+        __syncwarp();
+        if (lane == 0) pipe::bar_arrive(sh.piece_full + slot);
+        if (left <= 0) break;
+        ++pi;
+        const int nq = nrow > kRows ? 2 : 1;
+        for (int b = 0; b < nq; ++b, ++n_q) {                   // only the rows that exist: a product's rows do not mix
+          const int buf = n_q & 1;
+          if (n_q >= 2 && !(ok = warp_wait(sh.q_empty + buf, ((n_q >> 1) - 1) & 1, quit))) break;
+          const uint32_t dst = base + buf * Shape::tile + panel;
+          const int here = nrow - b * kRows < kRows ? nrow - b * kRows : kRows;
+          const char* from = a.q + (int64_t)w.g.tok * a.q_pitch + (int64_t)(w.g.kh * a.group) * a.q_head + ch * 16;
+#pragma unroll 2
+          for (int rr = sub; rr < here; rr += RI) {
+            const int x = w.g.blk * kBlock + b * kRows + rr;
+            const int jt = (int)a.group_div.div((uint32_t)x);
+            if (in_dim)
+              tc::copy16(dst + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4),
+                         from + jt * a.q_pitch + (x - jt * a.group) * a.q_head, true);
+          }
+          tc::copy_commit();
+          tc::copy_wait<0>();
+          tc::fence_async();
+          __syncwarp();
+          if (lane == 0) pipe::bar_arrive(sh.q_full + buf);
         }
         if (!ok) break;
-        if (tc::elect())
-          for (int b = 0; b < nq; ++b) tc::commit(sh.q_empty + ((n_q + b) & 1));
-        __syncwarp();
-        n_q += nq;
-        pos = next_pos<ST>(pos, n);
-        ++n_piece;
-        left -= n;
-        if (left <= 0) break;
-        off = 0;
-        w.next();
+        left -= units - y;
+        at += units;
+        y = 0;
+        if (left > 0) w.next();
       }
-    } else {
-      // ----------------------------------------------------------- loads ----
-      constexpr int CH = DP / 8, PN = DP / 64;                  // 16-byte chunks and 64-value panels of a row
-      constexpr uint32_t kPanel = kRows * 128;
-      const uint32_t base = tc::smem_addr(smem), ring = base + 2 * Shape::tile;
-      if (warp == 9) {
-        // keys and values: whole pages as boxes; a tile with a page that is cut
-        // short, or outside the pool, row by row, four rows at a time, with zeros
-        // for what is not there (a slot behind the end may hold anything)
-        if (lane < 2) {
-          tc::prefetch_map(maps.box + lane);
-          tc::prefetch_map(maps.row + lane);
-        }
-        const int none = (int)a.pool_rows;                      // a row outside the map
-        uint32_t pos = 0;
-        bool ok = true;
-        while (ok) {
-          const int n = (int)(w.g.tiles - off < left ? w.g.tiles - off : left);
-          const int np = w.prefix_part();
-          const int64_t own = w.own_keys();
-          for (int i = 0; i < n && ok; ++i) {
-            const int ti = off + i;
-            const bool pre = ti < np;
-            const int64_t key0 = (int64_t)(pre ? ti : ti - np) * kKeys;
-            const int64_t rest = (pre ? a.prefix_len : own) - key0;
-            const int valid = rest < 0 ? 0 : (rest < kKeys ? (int)rest : kKeys);
-            const int shift = pre ? 0 : a.prefix_len;           // own keys follow the prefix
-            bool boxes = p.run > 0 && valid == kKeys;
-            if (boxes) {
-              int32_t y = 0;
-              if (lane * p.run < kKeys) {
-                const int64_t sl = key_slot(a, w.g.req, (int32_t)key0 + lane * p.run + shift);
-                y = sl < 0 || sl + p.run > a.pool_rows ? -1 : (int32_t)sl;
-                sh.rows[lane] = y;
-              }
-              boxes = !__any_sync(0xffffffffu, y < 0);
-            }
-            if (!boxes) {
-              int4 y = make_int4(none, none, none, none);
-              int32_t* e = &y.x;
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (lane * 4 + j < valid) {
-                  const int64_t sl = key_slot(a, w.g.req, (int32_t)key0 + lane * 4 + j + shift);
-                  if (sl >= 0) e[j] = (int32_t)sl;
-                }
-              *reinterpret_cast<int4*>(sh.rows + lane * 4) = y;
-            }
-            __syncwarp();
-            for (int kv = 0; kv < 2; ++kv, ++pos) {
-              const uint32_t st = pos % ST;
-              if (pos >= ST && !(ok = warp_wait(sh.empty + st, (pos / ST - 1) & 1, quit))) break;
-              if (tc::elect()) {
-                pipe::bar_expect_tx(sh.full + st, Shape::tile);
-                const uint32_t dst = ring + st * Shape::tile;
-                const int x = w.g.kh * a.dim;
-                if (boxes) {
-                  const int nb = kKeys / p.run;
-#pragma unroll 2
-                  for (int b = 0; b < nb; ++b) {
-                    const int y = sh.rows[b];
-#pragma unroll
-                    for (int pn = 0; pn < PN; ++pn)
-                      tc::load_box(dst + pn * kPanel + b * p.run * 128, maps.box + kv, x + pn * 64, y, sh.full + st);
-                  }
-                } else {
-#pragma unroll 2
-                  for (int b = 0; b < kKeys / 4; ++b) {
-                    const int4 y = *reinterpret_cast<const int4*>(sh.rows + b * 4);
-#pragma unroll
-                    for (int pn = 0; pn < PN; ++pn)
-                      tc::load_rows(dst + pn * kPanel + b * 512, maps.row + kv, x + pn * 64, y, sh.full + st);
-                  }
-                }
-              }
-              __syncwarp();
-            }
-            if (pos >= kTurn<ST>) pos -= kTurn<ST> - ST * 2;  // keeps stage and parity, and counts as a full ring
-          }
-          left -= n;
-          if (left <= 0) break;
-          off = 0;
-          w.next();
-        }
-        // copies must not outlive the CTA: all are waited for by the products, unless a wait gave up
-        if (*quit)
-          for (uint32_t q = pos > ST ? pos - ST : 0; q < pos; ++q) (void)pipe::bar_wait(sh.full + q % ST, (q / ST) & 1);
-      } else {
-        // queries: only the rows that exist (a product's rows do not mix)
-        constexpr int RI = 32 / CH;                             // rows per instruction
-        const int lw = warp - 10, ch = lane % CH, sub = lane / CH;
-        const bool in_dim = ch * 8 < a.dim;
-        const uint32_t panel = (uint32_t)(ch >> 3) * kPanel;
-        uint32_t n_q = 0;
-        bool ok = true;
-        while (ok) {
-          const int rows = w.rows(), n = (int)(w.g.tiles - off < left ? w.g.tiles - off : left);
-          const int nq = rows > kRows ? 2 : 1;
-          for (int b = 0; b < nq; ++b, ++n_q) {
-            const int buf = n_q & 1;
-            if (n_q >= 2 && !(ok = warp_wait(sh.q_empty + buf, ((n_q >> 1) - 1) & 1, quit))) break;
-            const uint32_t dst = base + buf * Shape::tile;
-            const int here = rows - b * kRows < kRows ? rows - b * kRows : kRows;
-#pragma unroll 4
-            for (int rr = lw * RI + sub; rr < here; rr += 2 * RI) {
-              const int x = w.g.blk * kBlock + b * kRows + rr;
-              const int jt = (int)a.group_div.div((uint32_t)x);
-              const char* src = a.q + ((int64_t)w.g.tok + jt) * a.q_pitch +
-                                (int64_t)(w.g.kh * a.group + x - jt * a.group) * a.q_head + ch * 16;
-              if (in_dim) tc::copy16(dst + panel + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4), src, true);
-            }
-            tc::copy_commit();
-            tc::copy_wait<0>();
-            tc::fence_async();
-            __syncwarp();
-            if (lane == 0) pipe::bar_arrive(sh.q_full + buf);
-          }
-          left -= n;
-          if (left <= 0) break;
-          off = 0;
-          w.next();
-        }
-      }
-    }
     }
   }
   // No product may be in flight when tensor memory is given back: the softmax
   // warps have waited for the last of them, unless a wait gave up.
-  if (warp == 8 && *quit && !(tc::smem_addr(smem) & 1023u)) {
-    if (lane == 0) {
-      tc::commit(&sh.halves_read);  // its count is 8: the wait below only bounds the time the products get
-      const uint64_t t0 = pipe::now_ns();
-      while (pipe::now_ns() - t0 < 1000000ull) {
-      }
+  if (warp == 8 && *quit) {
+    const uint64_t t0 = pipe::now_ns();
+    while (pipe::now_ns() - t0 < 1000000ull) {
     }
     __syncwarp();
   }
@@ -868,145 +1036,143 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
 }
 
 // ------------------------------------------------------------ joining parts ---
-// Row (token, head): o = sum w_k o_k / sum w_k, w_k = 2^(lse_k - max lse), over
-// the parts of its prefix segment and of its own segment. Rows of uncut segments
-// without a second part have been written already. W warps share a row: a cut
-// segment can have as many parts as there are CTAs.
+// Row: o = sum w_k o_k / sum w_k, w_k = 2^(lse_k - max lse) over its parts.
+struct Sum {
+  float m = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ void add(float4 v, float ls) {
+    if (ls == -INFINITY) return;
+    const float top = fmaxf(m, ls), f = m == -INFINITY ? 0.f : tc::ex2(m - top), g = tc::ex2(ls - top);
+    l = (l == l ? l * f : l) + g;
+    m = top;
+    x[0] = x[0] * f + v.x * g;
+    x[1] = x[1] * f + v.y * g;
+    x[2] = x[2] * f + v.z * g;
+    x[3] = x[3] * f + v.w * g;
+  }
+};
+
+__device__ __forceinline__ float4 row4(const float* o, int dim, int lane) {
+  return lane * 4 < dim ? __ldg(reinterpret_cast<const float4*>(o) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+}
+
+// Adds every step-th part of row `brow` of a segment cut over CTAs c0 .. c1.
+__device__ __forceinline__ void add_cuts(Sum& sum, const TilePlan& p, int dim, int c0, int c1, int brow, int k0, int step,
+                                         int lane) {
+#pragma unroll 4
+  for (int c = c0 + k0; c <= c1; c += step) {
+    const int slot = 2 * c + (c == c0 ? 1 : 0);
+    const int64_t row = (int64_t)slot * kBlock + brow;
+    const int used = __ldg(p.used + slot);  // a stretch so short that no tile begins in it leaves none
+    const float4 v = row4(p.cut + row * dim, dim, lane);
+    const float ls = __ldg(p.cut_lse + row);
+    if (used) sum.add(v, ls);
+  }
+}
+
+// The block's eight warps' sums of one row, in warp 0.
+__device__ __forceinline__ void sum_warps(Sum& s, int warp, int lane) {
+  __shared__ float s_m[8], s_l[8], s_o[8][128];
+  if (lane == 0) {
+    s_m[warp] = s.m;
+    s_l[warp] = s.l;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) s_o[warp][lane * 4 + e] = s.x[e];
+  __syncthreads();
+  if (warp != 0) return;
+  float top = s.m;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) top = fmaxf(top, s_m[k]);
+  float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float f = s_m[k] == -INFINITY ? 0.f : tc::ex2(s_m[k] - top);
+    l += s_l[k] == s_l[k] ? s_l[k] * f : s_l[k];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] += s_o[k][lane * 4 + e] * f;
+  }
+  s.m = top;
+  s.l = l;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) s.x[e] = x[e];
+}
+
+template <typename T>
+__device__ __forceinline__ void write_row(const AttnArgs& a, int64_t grow, const Sum& s, int lane) {
+  const float inv = s.l == 0.f ? 0.f : 1.f / s.l;
+  if (lane * 4 < a.dim)
+    *reinterpret_cast<uint2*>(a.out + (grow * a.dim + lane * 4) * 2) =
+        make_uint2(Vec16<T>::pack2(s.x[0] * inv, s.x[1] * inv), Vec16<T>::pack2(s.x[2] * inv, s.x[3] * inv));
+  if (lane == 0 && a.lse) a.lse[grow] = s.l == 0.f ? -INFINITY : (s.m + log2f(s.l)) * 0.6931471805599453f;
+}
+
+// Rows with one segment each (prefix and own keys in one, or no prefix): only
+// those of cut segments. Block (c, i) does the share i of the rows of the cut
+// segment that ends in CTA c's stretch.
+template <typename T>
+__global__ void __launch_bounds__(256) attend_join_cuts_kernel(const AttnArgs a, const TilePlan p) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x;
+  const CutEnd e = p.end[c];
+  if (e.nrow == 0) return;
+  // few rows, maybe with many parts: a block to a row, a warp to an eighth of the parts
+  const bool split = e.nrow <= (int)gridDim.y;
+  for (int brow = split ? blockIdx.y : blockIdx.y * 8 + warp; brow < e.nrow; brow += gridDim.y * 8) {
+    const int x = e.x0 + brow, jt = (int)a.group_div.div((uint32_t)x);
+    const int64_t grow = ((int64_t)e.tok + jt) * a.hq + e.kh * a.group + (x - jt * a.group);
+    Sum s;
+    add_cuts(s, p, a.dim, e.c0, c, brow, split ? warp : 0, split ? 8 : 1, lane);
+    if (split) {
+      sum_warps(s, warp, lane);
+      if (warp != 0) return;
+    }
+    write_row<T>(a, grow, s, lane);
+  }
+}
+
+// Rows with a part over the prefix and a part over their own keys. W warps share
+// a row.
 template <typename T, int W>
 __global__ void __launch_bounds__(256) attend_join_kernel(const AttnArgs a, const TilePlan p) {
   grid_dep_wait();
   grid_dep_launch();
-  __shared__ float s_m[8], s_l[8], s_o[8][128];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t grow = (int64_t)blockIdx.x * (8 / W) + warp / W;
-  const int live = live_tokens(a), part = warp % W;
-  const int64_t rows = (int64_t)live * a.hq;
-  int n0 = 0, n1 = 0;          // parts of the prefix segment, of the own segment
-  int64_t c0[2] = {0, 0};      // their first CTA
-  int brow[2] = {0, 0};        // row in the block
-  bool cut0 = false, cut1 = false;
-  if (grow < rows) {
-    const int t = (int)(grow / a.hq), h = (int)(grow - (int64_t)t * a.hq);
-    const int kh = (int)a.group_div.div((uint32_t)h), gi = h - kh * a.group;
-    const int64_t total = __ldg(p.start + a.batch), unit = share(total, p.ctas);
-    Walk w(a, p, live);
-    const int pk = w.prefix_keys();
-    if (pk > 0) {
-      w.prefix_space();
-      const int64_t x = (int64_t)t * a.group + gi;
-      const int tp = tile_count(a.prefix_len), blk = (int)(x / kBlock);
-      const int64_t s = ((int64_t)kh * w.g.nblk + blk) * tp, e = s + tp - 1;
-      c0[0] = s / unit;
-      n0 = (int)(e / unit - c0[0]) + 1;
-      cut0 = n0 > 1;
-      brow[0] = (int)(x - (int64_t)blk * kBlock);
-    }
-    int r = 0, hi = a.batch;   // the last r with cu[r] <= t
-    while (hi - r > 1) {
-      const int mid = (r + hi) >> 1;
-      if (__ldg(a.cu + mid) <= t)
-        r = mid;
-      else
-        hi = mid;
-    }
-    w.request(r);
-    if (t >= w.g.tok && t < w.g.tok + w.g.ntok) {
-      const int64_t x = (int64_t)(t - w.g.tok) * a.group + gi;
-      const int blk = (int)(x / kBlock);
-      int64_t before = 0, one = 0, here = 0;  // tiles of the blocks before this one, of all, of this one
-      for (int b = lane; b < w.g.nblk; b += 32) {
-        w.g.blk = b;
-        const int n = w.block_tiles();
-        one += n;
-        if (b < blk) before += n;
-        if (b == blk) here = n;
-      }
-#pragma unroll
-      for (int d = 16; d; d >>= 1) {
-        one += __shfl_xor_sync(0xffffffffu, one, d);
-        before += __shfl_xor_sync(0xffffffffu, before, d);
-        here += __shfl_xor_sync(0xffffffffu, here, d);
-      }
-      const int64_t s = __ldg(p.start + r) + kh * one + before, e = s + here - 1;
-      c0[1] = s / unit;
-      n1 = (int)(e / unit - c0[1]) + 1;
-      cut1 = n1 > 1;
-      brow[1] = (int)(x - (int64_t)blk * kBlock);
-    }
-  }
-  const int n = n0 + n1;
-  const bool on = n > 1 || (n == 1 && !p.joint && a.prefix_len > 0);
-  const auto locate = [&](int k, const float*& o, float& ls) {
-    const int u = k < n0 ? 0 : 1, i = u ? k - n0 : k;
-    if (u ? cut1 : cut0) {
-      // its first part is the last stretch of its first CTA, the others first stretches
-      const int64_t row = (2 * (c0[u] + i) + (i == 0 ? 1 : 0)) * kBlock + brow[u];
-      o = p.cut + row * a.dim;
-      ls = __ldg(p.cut_lse + row);
-    } else {
-      const int64_t row = (u ? a.tokens * a.hq : 0) + grow;
-      o = p.whole + row * a.dim;
-      ls = __ldg(p.whole_lse + row);
-    }
-  };
-  float m = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % W;
+  const int64_t grow = (int64_t)blockIdx.x * (8 / W) + warp / W, all = a.tokens * a.hq;
+  const bool on = grow < (int64_t)live_tokens(a) * a.hq;
+  Sum sum;
   if (on) {
-    for (int k = part; k < n; k += W) {
-      const float* o;
-      float ls;
-      locate(k, o, ls);
-      if (ls == -INFINITY) continue;
-      const float top = fmaxf(m, ls), f = m == -INFINITY ? 0.f : tc::ex2(m - top), g = tc::ex2(ls - top);
-      l = l * f + g;
-      m = top;
-      if (lane * 4 < a.dim) {
-        const float4 v = __ldg(reinterpret_cast<const float4*>(o) + lane);
-        x[0] = x[0] * f + v.x * g;
-        x[1] = x[1] * f + v.y * g;
-        x[2] = x[2] * f + v.z * g;
-        x[3] = x[3] * f + v.w * g;
+    const int2 at[2] = {__ldg(p.place + grow), __ldg(p.place + all + grow)};
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      // the own keys' parts start with the last warp, the prefix's with the first
+      const int k0 = u ? W - 1 - part : part;
+      if (at[u].x < 0) {
+        if (k0 == 0) sum.add(row4(p.whole + (u * all + grow) * a.dim, a.dim, lane), __ldg(p.whole_lse + u * all + grow));
+      } else {
+        // (a token that the batch's offsets leave out has no place: what is read stays inside the workspace)
+        const int c0 = (at[u].x & 0xffff) < p.ctas ? at[u].x & 0xffff : 0, c1 = at[u].y < p.ctas ? at[u].y : 0;
+        add_cuts(sum, p, a.dim, c0, c1, (at[u].x >> 16) & (kBlock - 1), k0, W, lane);
       }
     }
   }
   if (W > 1) {
-    s_m[warp] = m;
-    s_l[warp] = l;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s_o[warp][lane * 4 + e] = x[e];
-    __syncthreads();
-    if (part != 0) return;
-    float top = m;
-    for (int k = 1; k < W; ++k) top = fmaxf(top, s_m[warp + k]);
-    float f = m == -INFINITY ? 0.f : tc::ex2(m - top);
-    l = l == l ? l * f : l;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] *= f;
-    for (int k = 1; k < W; ++k) {
-      f = s_m[warp + k] == -INFINITY ? 0.f : tc::ex2(s_m[warp + k] - top);
-      l += s_l[warp + k] == s_l[warp + k] ? s_l[warp + k] * f : s_l[warp + k];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] += s_o[warp + k][lane * 4 + e] * f;
-    }
-    m = top;
+    sum_warps(sum, warp, lane);
+    if (warp != 0) return;
   }
-  if (!on) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (lane * 4 < a.dim) {
-    const uint2 v = make_uint2(Vec16<T>::pack2(x[0] * inv, x[1] * inv), Vec16<T>::pack2(x[2] * inv, x[3] * inv));
-    *reinterpret_cast<uint2*>(a.out + (grow * a.dim + lane * 4) * 2) = v;
-  }
-  if (lane == 0 && a.lse) a.lse[grow] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  if (on) write_row<T>(a, grow, sum, lane);
 }
 
 // The tensor core takes 16-bit values, sixteen at a time; a head of more than
 // 128 of them, of an odd half of sixteen, or of 32-bit values goes row by row.
+// So does a scale next to nothing, under which a masked score would not vanish.
 bool takes_tiles(const AttnArgs& a, int dtype) {
-  return dtype != GSEC_F32 && a.dim <= 128 && a.dim % 16 == 0;
+  return dtype != GSEC_F32 && a.dim <= 128 && a.dim % 16 == 0 && !(fabsf(a.scale) < 1e-20f);
 }
 
 // Stacking the requests' rows over the prefix pays when they would not fill
 // tiles by themselves; with about a tile of rows each (or one request) prefix and
-// own keys are better taken in one go, which leaves nothing to join.
+// own keys are better taken in one go, which leaves little to join.
 TilePlan tile_plan(const AttnArgs& a, int64_t* bytes) {
   TilePlan p{};
   p.ctas = sm_count();
@@ -1020,7 +1186,9 @@ TilePlan tile_plan(const AttnArgs& a, int64_t* bytes) {
     return x;
   };
   const int64_t rows = a.tokens * a.hq, parts = p.joint ? 0 : 2;
-  p.start = reinterpret_cast<int64_t*>(take((a.batch + 1) * 8));
+  p.used = reinterpret_cast<int32_t*>(take((int64_t)2 * p.ctas * 4));
+  p.end = reinterpret_cast<CutEnd*>(take(p.ctas * (int64_t)sizeof(CutEnd)));
+  p.place = reinterpret_cast<int2*>(take(parts * rows * 8));
   p.whole_lse = reinterpret_cast<float*>(take(parts * rows * 4));
   p.cut_lse = reinterpret_cast<float*>(take((int64_t)2 * p.ctas * kBlock * 4));
   p.whole = reinterpret_cast<float*>(take(parts * rows * a.dim * 4));
@@ -1062,12 +1230,20 @@ template <typename T, int DP>
 int launch_tiles(const AttnArgs& a, cudaStream_t s) {
   int64_t bytes = 0;
   const TilePlan p = tile_plan(a, &bytes);
+  // the line is counted in 32 bits
+  const int64_t keys = (int64_t)a.prefix_len + (int64_t)a.width * a.page;
+  const int64_t blocks = a.tokens * a.group / kBlock + a.batch + 1;  // of the requests, and of the prefix
+  GSEC_REQUIRE((double)blocks * 2 * a.hk * ((keys / kKeys + 3.0) * kUnitTile + kUnitSegment) < 2.0e9 &&
+                   a.tokens * a.group < (1ll << 30),
+               "prefix_attention: %lld tokens on %lld keys are too many for one call", (long long)a.tokens,
+               (long long)keys);
   PoolMaps maps;
   bool ok = true;
   for (int kv = 0; kv < 2; ++kv) {
     const char* at = a.pool + (kv ? a.plane : 0);
-    ok = ok && pool_map(maps.box + kv, Vec16<T>::bf16, at, (int64_t)a.hk * a.dim, a.pool_rows, a.pitch, p.run ? p.run : 1) &&
-         pool_map(maps.row + kv, Vec16<T>::bf16, at, (int64_t)a.hk * a.dim, a.pool_rows, a.pitch, 1);
+    const int64_t values = (int64_t)a.hk * a.dim;
+    ok = ok && pool_map(maps.box + kv, Vec16<T>::bf16, at, values, a.pool_rows, a.pitch, p.run ? p.run : 1) &&
+         pool_map(maps.row + kv, Vec16<T>::bf16, at, values, a.pool_rows, a.pitch, 1);
   }
   if (!ok) {
     set_error("prefix_attention: the pool's tensor maps were refused");
@@ -1076,15 +1252,13 @@ int launch_tiles(const AttnArgs& a, cudaStream_t s) {
   constexpr int smem = TileShape<DP>::smem;
   if (launch_cache().blocks_per_sm(attend_tile_kernel<T, DP>, kTileThreads, smem) < 0)
     return check_launch("attend_tile launch shape");
-  // a smaller launch would leave the softmax warpgroups waiting for registers that are not there
-  static const bool regs_ok = [] {
-    cudaFuncAttributes at{};
-    return cudaFuncGetAttributes(&at, attend_tile_kernel<T, DP>) == cudaSuccess && at.numRegs == kLaunchRegs;
-  }();
-  GSEC_REQUIRE(regs_ok, "attend_tile: launch registers are not %d", kLaunchRegs);
-  const int rc = launch_rc(launch_pdl(attend_tile_kernel<T, DP>, dim3((unsigned)p.ctas), dim3(kTileThreads), smem, s, a, p, maps),
-                           "prefix_attention");
+  const int rc = launch_rc(
+      launch_pdl(attend_tile_kernel<T, DP>, dim3((unsigned)p.ctas), dim3(kTileThreads), smem, s, a, p, maps),
+      "prefix_attention");
   if (rc) return rc;
+  if (p.joint)
+    return launch_rc(launch_pdl(attend_join_cuts_kernel<T>, dim3((unsigned)p.ctas, 8), dim3(256), 0, s, a, p),
+                     "prefix_attention join");
   const int64_t rows = a.tokens * a.hq;
   // few rows: eight warps to a row, since each may have a part from every CTA
   if (rows <= (int64_t)p.ctas * 16)
