@@ -163,11 +163,8 @@ int attend_rows(const AttnArgs& a, cudaStream_t s) {
 // new tokens. A block is up to 256 such rows of one KV head; a segment is a block
 // with its keys, cut into tiles of 128. Scores S = Q K^T (128 x 128) and O += P V
 // run on the tensor core with S, P and O in tensor memory; one thread holds one
-// row, keeps its maximum m and sum l in registers, and replaces S by
-// P = 2^(S c - m c) in place. O is scaled by 2^(m_old - m) only when the maximum
-// has grown by more than 8 binary places since P was last taken relative to it;
-// until then P exceeds 1 by at most 2^8, which fp32 sums and 16-bit P hold as
-// well as they hold 1.
+// row, keeps its reference m and sum l in registers, and replaces S by
+// P = 2^(S c - m c) in place.
 //
 // Two warpgroups take turns, so that one's exponentials run under the other's
 // products. A tile of a block with more than 128 rows is two steps, one for each
@@ -186,11 +183,15 @@ int attend_rows(const AttnArgs& a, cudaStream_t s) {
 // line is one warp's work, which hands the pieces to the others through shared
 // memory, and loops are unrolled only as far as they have to be (with the walk in
 // every role and 128-column bodies a one-tile segment took 12000 cycles).
-constexpr int kTileThreads = 384;   // 2 softmax warpgroups; issue products, load K, load V, walk and load Q: a warp each
+constexpr int kTileThreads = 384;   // 2 softmax warpgroups; 2 warps issue products, 1 loads K and V, 1 walks and loads Q
 constexpr int kRows = 128, kKeys = 128, kBlock = 256;
 // Units of the line: a tile of a whole block; half a block's tile is three
 // quarters of that; a segment's beginning and end.
 constexpr int kUnitTile = 32, kUnitSegment = 16;
+// Registers: a softmax thread holds 64 scores and 64 words of P. The launch has 168
+// per thread; the third warpgroup hands over what it does not need.
+constexpr int kLaunchRegs = 168, kSoftmaxRegs = 200, kOtherRegs = 104;
+static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * kLaunchRegs, "register shares");
 constexpr int kMinShare = 64;       // a stretch is at least about two tiles
 
 // A block and its keys: rows [blk * kBlock, ...) of the row space that starts at
@@ -209,6 +210,8 @@ struct Start {           // a point on the line
 
 struct TilePlan {
   int run;               // rows of a box: the largest power of two dividing the page, at most a tile; 0: rows one by one
+  int run_log;
+  int slope;             // units by which a request's blocks grow
   int joint;             // prefix and own keys of a request are one segment (no stacking over requests)
   int ctas;
   // rows of uncut segments (0 prefix, 1 own) that have another part
@@ -301,10 +304,7 @@ struct Walk {
     const int more = g.len - g.ntok;
     return prefix_part() * kUnitTile + (more > 0 ? more / (kKeys / kUnitTile) : 0);
   }
-  __device__ __forceinline__ int slope() const {
-    const int s = kBlock / (kKeys / kUnitTile) / a.group;
-    return g.req < 0 ? 0 : (s > 0 ? s : 1);
-  }
+  __device__ __forceinline__ int slope() const { return g.req < 0 ? 0 : p.slope; }
   __device__ __forceinline__ int units() const {
     const int u = base_units() + slope() * (g.blk + 1);
     return kUnitSegment + (pair() ? u : u - u / 4);
@@ -394,22 +394,21 @@ __device__ __forceinline__ int share(int total, int ctas) {
   return n < kMinShare ? kMinShare : n;
 }
 
-// A wait that gives up raises `quit`, which ends every other wait of the CTA.
+// A wait gives up after 2^24 turns (about a second) and raises `quit`, which ends
+// every other wait of the CTA.
+__device__ __forceinline__ bool thread_wait(uint64_t* bar, uint32_t parity, volatile int* quit) {
+#pragma unroll 1
+  for (int i = 0; i < 1 << 24; ++i) {
+    if (pipe::bar_try(bar, parity)) return true;
+    if (*quit) return false;
+  }
+  *quit = 1;
+  atomicOr(&g_attn_status, 2u);
+  return false;
+}
 // Every lane of the warp gets the same answer.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* quit) {
-  bool ok = pipe::bar_try(bar, parity);
-  if (!__all_sync(0xffffffffu, ok)) {
-    const uint64_t t0 = pipe::now_ns();
-    while (!ok && !(ok = pipe::bar_try(bar, parity))) {
-      if (*quit) break;
-      if (pipe::now_ns() - t0 > pipe::kWaitNs) {
-        *quit = 1;
-        atomicOr(&g_attn_status, 2u);
-        break;
-      }
-    }
-  }
-  return __all_sync(0xffffffffu, ok) != 0;
+  return __all_sync(0xffffffffu, thread_wait(bar, parity, quit)) != 0;
 }
 
 template <int DP>
@@ -423,7 +422,7 @@ struct TileShape {
 // Shared memory behind the tiles.
 struct TileShared {
   float m[kRows], l[kRows];         // what one warpgroup hands to the other
-  alignas(16) int32_t rows[2][kKeys];  // pool rows of the K and the V tile being loaded
+  alignas(16) int32_t rows[kKeys];  // pool rows of the tile being loaded
   uint64_t full[12], empty[12], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], o_empty[2], handed, taken;
   uint64_t piece_full[kPieces], piece_empty[kPieces];
   Piece piece[kPieces];
@@ -449,78 +448,108 @@ __device__ __forceinline__ void mask_tile(uint32_t ts, int cols) {
   tc::wait_st();
 }
 
-__device__ __forceinline__ float max32(const uint32_t* x, float m) {
-  float t[2] = {m, m};
-#pragma unroll
-  for (int e = 0; e < 32; e += 4) {
-    t[0] = fmaxf(fmaxf(t[0], __uint_as_float(x[e])), __uint_as_float(x[e + 1]));
-    t[1] = fmaxf(fmaxf(t[1], __uint_as_float(x[e + 2])), __uint_as_float(x[e + 3]));
-  }
-  return fmaxf(t[0], t[1]);
-}
-
-// 32 scores become 16 words of P; returns their sum.
+// 16 words of P from 32 scores, their sum and their maximum (with `top`). (Two
+// scores to an instruction, fma.f32x2 and add.f32x2, took longer: 1550 cycles a
+// tile instead of 1290.)
 template <typename T>
-__device__ __forceinline__ float exp32(uint32_t* x, float c, float mc) {
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+__device__ __forceinline__ float exp32(const uint32_t* x, uint32_t* w, float c, float mc, float& top) {
+  float sum[4] = {0.f, 0.f, 0.f, 0.f}, t[2] = {top, top};
 #pragma unroll
   for (int e = 0; e < 32; e += 2) {
-    const float p0 = tc::ex2(fmaf(__uint_as_float(x[e]), c, -mc)), p1 = tc::ex2(fmaf(__uint_as_float(x[e + 1]), c, -mc));
+    const float s0 = __uint_as_float(x[e]), s1 = __uint_as_float(x[e + 1]);
+    const float p0 = tc::ex2(fmaf(s0, c, -mc)), p1 = tc::ex2(fmaf(s1, c, -mc));
     sum[(e >> 1) & 3] += p0 + p1;
-    x[e >> 1] = Vec16<T>::pack2(p0, p1);
+    t[(e >> 1) & 1] = fmaxf(fmaxf(t[(e >> 1) & 1], s0), s1);
+    w[e >> 1] = Vec16<T>::pack2(p0, p1);
   }
+  top = fmaxf(t[0], t[1]);
   return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
-// One row's share of a tile: the scores at tensor memory `ts` (128 columns) become
-// 16-bit P there; (m, l) follow, and O at `to` (when it holds something) is
-// brought to the new reference. What a lane without a row (!on) computes is not
-// read. The scores are read twice, 64 columns at a time: that costs less than
-// the registers and the code of 128 at once.
+// A tile whose maximum moves the reference of some row of the warp (or gives it
+// one): maximum first, then O and l to the new reference, then P.
 template <typename T, int DP>
-__device__ __forceinline__ void softmax_tile(uint32_t ts, uint32_t to, float c, bool on, bool has_o, float& m, float& l) {
-  uint32_t x[32], y[32];
+__device__ __noinline__ float2 move_and_softmax(uint32_t ts, uint32_t to, float c, bool on, bool has_o, float m, float l) {
+  uint32_t x[32], w[16];
   float top = m;
 #pragma unroll 1
-  for (int k = 0; k < 128; k += 64) {
+  for (int k = 0; k < 128; k += 32) {
     tc::ld32(ts + k, x);
-    tc::ld32(ts + k + 32, y);
     tc::wait_ld(x);
-    tc::wait_ld(y);
-    top = max32(y, max32(x, top));
-  }
-  // move the reference when it is too far behind (or there is none yet)
-  const bool move = on && ((top - m) * c > 8.f || (m == -INFINITY && top > -INFINITY));
-  if (__any_sync(0xffffffffu, move)) {
-    const float f = !move ? 1.f : (m == -INFINITY ? 0.f : tc::ex2((m - top) * c));
-    if (move) m = top;
-    l *= f;
-    if (has_o) {
-#pragma unroll 1
-      for (int k = 0; k < DP; k += 32) {
-        tc::ld32(to + k, x);
-        tc::wait_ld(x);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
-        tc::st32(to + k, x);
-      }
+    for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(x[e]));
+  }
+  const bool move = on && ((top - m) * c > 8.f || (m == -INFINITY && top > -INFINITY));
+  const float f = !move ? 1.f : (m == -INFINITY ? 0.f : tc::ex2((m - top) * c));
+  if (move) m = top;
+  l *= f;
+  if (has_o) {
+#pragma unroll 1
+    for (int k = 0; k < DP; k += 32) {
+      tc::ld32(to + k, x);
+      tc::wait_ld(x);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+      tc::st32(to + k, x);
     }
   }
   const float mc = m == -INFINITY ? 0.f : m * c;
-  // P's words overlay the scores from the left: 32 columns of scores are read before the 16 words go out
-  tc::ld32(ts, x);
+  float seen = -INFINITY;
+  // P's words overlay the scores from the left, behind the reading
 #pragma unroll 1
-  for (int k = 0; k < 128; k += 64) {
+  for (int k = 0; k < 128; k += 32) {
+    tc::ld32(ts + k, x);
     tc::wait_ld(x);
-    tc::ld32(ts + k + 32, y);
-    l += exp32<T>(x, c, mc);
-    tc::wait_ld(y);
-    tc::st16(ts + k / 2, x);
-    if (k == 0) tc::ld32(ts + 64, x);
-    l += exp32<T>(y, c, mc);
-    tc::st16(ts + k / 2 + 16, y);
+    l += exp32<T>(x, w, c, mc, seen);
+    tc::st16(ts + k / 2, w);
   }
   tc::wait_st();
+  return make_float2(m, l);
+}
+
+// One row's share of a tile: the scores at tensor memory `ts` (128 columns) become
+// 16-bit P there, (m, l) follow, and O at `to` (when it holds something) where the
+// reference moves. What a lane without a row (!on) computes is not read.
+//
+// P is taken relative to the reference m that the row has, while the tile's
+// maximum is found on the way: one pass over the scores, and no branch in it, so
+// that the exponentials of one part run under the loads, sums and conversions of
+// another (1300 cycles; 1900 in a loop over 64 columns; 1024 are the exponentials).
+// Only where the maximum turns out 8 binary places ahead, or the row has no
+// reference yet, is the reference moved and the tile done again; until then P
+// exceeds 1, by 2^8 at most, which sums and 16-bit P hold as well as they hold 1.
+template <typename T, int DP>
+__device__ __forceinline__ void softmax_tile(uint32_t ts, uint32_t to, float c, bool on, bool has_o, float& m, float& l) {
+  bool again = __any_sync(0xffffffffu, on && m == -INFINITY);
+  if (!again) {
+    uint32_t x[32], y[32], w[64];
+    const float mc = m == -INFINITY ? 0.f : m * c;
+    float top = m, sum;
+    tc::ld32(ts, x);
+    tc::wait_ld(x);
+    tc::ld32(ts + 32, y);
+    sum = exp32<T>(x, w, c, mc, top);
+    tc::wait_ld(y);
+    tc::ld32(ts + 64, x);
+    sum += exp32<T>(y, w + 16, c, mc, top);
+    tc::wait_ld(x);
+    tc::ld32(ts + 96, y);
+    sum += exp32<T>(x, w + 32, c, mc, top);
+    tc::wait_ld(y);
+    sum += exp32<T>(y, w + 48, c, mc, top);
+    again = __any_sync(0xffffffffu, on && (top - m) * c > 8.f);
+    if (!again) {
+      l += sum;
+      tc::st32(ts, w);
+      tc::st32(ts + 32, w + 32);
+      tc::wait_st();
+    }
+  }
+  if (again) {
+    const float2 r = move_and_softmax<T, DP>(ts, to, c, on, has_o, m, l);
+    m = r.x;
+    l = r.y;
+  }
 }
 
 template <typename T, int DP>
@@ -534,11 +563,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
   if (tid == 0) {
     for (int i = 0; i < (int)ST; ++i) {
       pipe::bar_init(sh.full + i, 1);
-      pipe::bar_init(sh.empty + i, 1);
+      pipe::bar_init(sh.empty + i, 2);  // both threads that issue products
     }
     for (int i = 0; i < 2; ++i) {
       pipe::bar_init(sh.q_full + i, 1);
-      pipe::bar_init(sh.q_empty + i, 1);
+      pipe::bar_init(sh.q_empty + i, 2);
       pipe::bar_init(sh.s_full + i, 1);
       pipe::bar_init(sh.p_full + i, 4);
       pipe::bar_init(sh.o_full + i, 1);
@@ -546,7 +575,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
     }
     for (int i = 0; i < kPieces; ++i) {
       pipe::bar_init(sh.piece_full + i, 1);
-      pipe::bar_init(sh.piece_empty + i, 12);  // 8 softmax warps, both loads, scores and sums of the products
+      pipe::bar_init(sh.piece_empty + i, 11);  // 8 softmax warps, the loads, both threads that issue products
     }
     pipe::bar_init(&sh.handed, 4);
     pipe::bar_init(&sh.taken, 4);
@@ -558,7 +587,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
     tc::alloc(&sh.tmem, 512);
     tc::relinquish();
   }
-  if (warp == 9 && lane < 2) {
+  if (warp == 10 && lane < 2) {
     tc::prefetch_map(maps.box + lane);
     tc::prefetch_map(maps.row + lane);
   }
@@ -640,6 +669,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
     };
     const uint32_t base = tc::smem_addr(smem), ring = base + 2 * Shape::tile;
     if (warp < 8) {
+      tc::regs_up<kSoftmaxRegs>();
       // ------------------------------------------------ softmax warpgroups ----
       const int t = warp >> 2, r = tid & (kRows - 1);
       const uint32_t row = (uint32_t)((warp & 3) * 32) << 16;
@@ -666,16 +696,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
         const int jt = (int)a.group_div.div((uint32_t)x);
         int see = g.more + jt + 1;
         see = see < 0 ? 0 : (see > g.len ? g.len : see);
-        float m = -INFINITY, l = 0.f;
+        float m = -INFINITY, l = 0.f;                          // reference, sum relative to it
         bool ok = true;
 #pragma unroll 1
         for (int i = two ? 0 : half; i < n; i += two ? 1 : 2) {
+          const int cols = on ? piece_keys(g, i, a.prefix_len, see) : kKeys;
+          const bool cut = __any_sync(0xffffffffu, cols < kKeys);
           if (!(ok = warp_wait(sh.s_full + t, n_s & 1, quit))) break;
           ++n_s;
           tc::fence_after();
           if (warp_on) {
-            const int cols = on ? piece_keys(g, i, a.prefix_len, see) : kKeys;
-            if (__any_sync(0xffffffffu, cols < kKeys)) mask_tile(ts, cols);
+            if (cut) mask_tile(ts, cols);
             softmax_tile<T, DP>(ts, to, c, on, two ? i > 0 : i >= 2, m, l);
           }
           tc::fence_before();
@@ -702,12 +733,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
           const float mb = sh.m[r], lb = sh.l[r];
           __syncwarp();
           if (lane == 0) pipe::bar_arrive(&sh.taken);
-          const float top = fmaxf(m, mb);
-          w0 = m == -INFINITY ? 0.f : tc::ex2((m - top) * c);
-          w1 = mb == -INFINITY ? 0.f : tc::ex2((mb - top) * c);
+          const float ref = fmaxf(m, mb);
+          w0 = m == -INFINITY ? 0.f : tc::ex2((m - ref) * c);
+          w1 = mb == -INFINITY ? 0.f : tc::ex2((mb - ref) * c);
           // a sum that is not a number stays so, whatever its maximum
           l = (l == l ? w0 * l : l) + (lb == lb ? w1 * lb : lb);
-          m = top;
+          m = ref;
           if (!warp_wait(sh.o_full + (t ^ 1), turn_other & 1, quit)) break;
         }
         if (!warp_wait(sh.o_full + t, turn & 1, quit)) break;
@@ -777,105 +808,107 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
         }
         done_piece(pi);
       }
-    } else if (warp == 8) {
+    } else {
+    tc::regs_down<kOtherRegs>();
+    if (warp < 10) {
       // -------------------------------------------------------- products ----
-      // The whole warp walks along; one lane issues. Step s runs on S, P and O
-      // number s & 1; its scores are issued right after the P V of step s - 2.
-      const uint32_t id_s = tc::idesc(Vec16<T>::bf16, kRows, 0, false, a.scale < 0.f);
-      const uint32_t id_o = tc::idesc(Vec16<T>::bf16, kRows, a.dim, true);
-      const int ks = a.dim / 16;
-      uint32_t n_p[2] = {0, 0}, n_o[2] = {0, 0}, n_q = 0;
-      // the scores' place: piece, tile, step of the tile; the sums' place
-      uint32_t qp = 0, qs = 0, qt = 0, wp = 0, wt = 0;
-      int qi = 0, qsub = 0, qn = 0, wn = 0;
-      bool qtwo = false, more = true;
-      const auto scores = [&]() {
-        if (!more) return true;
-        if (qi == 0 && qsub == 0) {
-          if (!next_piece(qp)) return false;
-          qn = sh.piece[qp % kPieces].n;
-          qtwo = sh.piece[qp % kPieces].nrow > kRows;
-          if (qn == 0) {
-            more = false;
-            return true;
+      // One thread for each warpgroup's steps. A step is P V of the last and Q K^T
+      // of the next of them, whose scores take the place of that P. Issuing is slow
+      // (64 cycles a product, the rate at which they run), and so is a lone thread's
+      // arithmetic (five cycles and more an instruction): with both in one thread
+      // the tensor core waited for every other step's preparation. Here one thread
+      // prepares while the other issues.
+      if (tc::elect()) {
+        const int t = warp - 8;
+        const uint32_t ts = tmem + t * 128;
+        const uint32_t id_s = tc::idesc(Vec16<T>::bf16, kRows, 0, false, a.scale < 0.f);
+        const uint32_t id_o = tc::idesc(Vec16<T>::bf16, kRows, a.dim, true);
+        const int ks = a.dim / 16;
+        const uint64_t qdesc = tc::desc(base, 16, 1024), kdesc = tc::desc(ring, 16, 1024),
+                       vdesc = tc::desc(ring, kKeys * 128, 1024);
+        uint32_t pi = 0, tiles = 0, n_q = 0, step = 0, n_p = 0, n_o = 0;  // pieces, tiles and Q tiles before this piece
+        int i = 0, n = 0, half = 0;
+        bool two = false;
+        // the step whose P is on its way: its V and what to do with O
+        bool have = false, fresh = false, last = false, alone = false;
+        uint32_t at = 0;
+        int kk = 0;
+        while (true) {
+          // the next step, if there is one
+          while (i >= n) {
+            if (n > 0) {
+              pipe::bar_arrive(sh.piece_empty + pi % kPieces);
+              ++pi;
+              tiles += n;
+              n_q += two ? 2 : 1;
+            }
+            if (!thread_wait(sh.piece_full + pi % kPieces, (pi / kPieces) & 1, quit)) break;
+            const Piece& g = sh.piece[pi % kPieces];
+            n = g.n;
+            if (n == 0) break;
+            two = g.nrow > kRows;
+            half = t ^ (int)(step & 1);
+            step += two ? 2 * n : n;
+            i = two ? 0 : half;
           }
-        }
-        const int l2 = qs & 1;
-        if (qi == 0 && !warp_wait(sh.q_full + ((n_q + qsub) & 1), ((n_q + qsub) >> 1) & 1, quit)) return false;
-        const uint32_t at = 2 * qt, st = at % ST;
-        if (!warp_wait(sh.full + st, (at / ST) & 1, quit)) return false;
-        tc::fence_after();
-        const Piece& g = sh.piece[qp % kPieces];
-        const uint32_t id = id_s | (uint32_t)(2 * sixteens(piece_keys(g, qi, a.prefix_len, g.own))) << 17;
-        const uint64_t qd = tc::desc(base + ((n_q + qsub) & 1) * Shape::tile, 16, 1024);
-        const uint64_t kd = tc::desc(ring + st * Shape::tile, 16, 1024);
-        const bool tile_done = !qtwo || qsub == 1, done = tile_done && qi == qn - 1;
-        if (tc::elect()) {
+          if (i >= n && n > 0) break;                           // a wait gave up
+          const bool more = n > 0;
+          const Piece& g = sh.piece[pi % kPieces];
+          const int qk = more ? sixteens(piece_keys(g, i, a.prefix_len, g.own)) : 0;
+          const uint32_t q_at = 2 * (tiles + i), q_st = q_at % ST, q_buf = n_q + (two ? half : 0);
+          const uint64_t qd = qdesc + (q_buf & 1) * (Shape::tile >> 4), kd = kdesc + q_st * (Shape::tile >> 4);
+          const bool q_first = i == (two ? 0 : half), q_last = i + (two ? 1 : 2) >= n;
+          if (more) {
+            if (q_first && !thread_wait(sh.q_full + (q_buf & 1), (q_buf >> 1) & 1, quit)) break;
+            if (!thread_wait(sh.full + q_st, (q_at / ST) & 1, quit)) break;
+          }
+          if (have) {
+            const uint32_t st = at % ST;
+            const uint64_t vd = vdesc + st * (Shape::tile >> 4);
+            if (!thread_wait(sh.full + st, (at / ST) & 1, quit)) break;
+            if (fresh && n_o > 0 && !thread_wait(sh.o_empty + t, (n_o - 1) & 1, quit)) break;
+            n_o += fresh;
+            if (!thread_wait(sh.p_full + t, n_p & 1, quit)) break;
+            ++n_p;
+            tc::fence_after();
+            if (kk == kKeys / 16) {
+#pragma unroll
+              for (int j = 0; j < kKeys / 16; ++j)
+                tc::mma_ts(ts + 256, ts + j * 8, vd + j * (2048 >> 4), id_o, !fresh || j > 0);
+            } else {
+#pragma unroll 1
+              for (int j = 0; j < kk; ++j) tc::mma_ts(ts + 256, ts + j * 8, vd + j * (2048 >> 4), id_o, !fresh || j > 0);
+            }
+            tc::commit(sh.empty + st);
+            if (alone) tc::commit(sh.empty + st);               // the other thread's arrival: it takes no part in the tile
+            if (last) tc::commit(sh.o_full + t);
+          }
+          if (!more) break;
+          if (!have) tc::fence_after();
+          const uint32_t id = id_s | (uint32_t)(2 * qk) << 17;
 #pragma unroll
           for (int j = 0; j < DP / 16; ++j) {
             const uint32_t o = ((j >> 2) * (kRows * 128) + (j & 3) * 32) >> 4;
-            if (j < ks) tc::mma_ss(tmem + l2 * 128, qd + o, kd + o, id, j > 0);
+            if (j < ks) tc::mma_ss(ts, qd + o, kd + o, id, j > 0);
           }
-          tc::commit(sh.s_full + l2);
-          if (tile_done) tc::commit(sh.empty + st);
-          if (done) {
-            tc::commit(sh.q_empty + (n_q & 1));
-            if (qtwo) tc::commit(sh.q_empty + ((n_q + 1) & 1));
+          tc::commit(sh.s_full + t);
+          tc::commit(sh.empty + q_st);
+          if (!two) tc::commit(sh.empty + q_st);
+          if (q_last) {
+            tc::commit(sh.q_empty + (q_buf & 1));
+            if (two || n == 1) tc::commit(sh.q_empty + (q_buf & 1));
           }
+          have = true;
+          fresh = q_first;
+          last = q_last;
+          alone = !two;
+          at = q_at + 1;
+          kk = qk;
+          i += two ? 1 : 2;
         }
-        __syncwarp();
-        ++qs;
-        qsub = tile_done ? 0 : 1;
-        if (tile_done) {
-          ++qt;
-          ++qi;
-        }
-        if (done) {
-          n_q += qtwo ? 2 : 1;
-          qi = 0;
-          done_piece(qp++);
-        }
-        return true;
-      };
-      bool ok = scores() && scores();
-      for (uint32_t s = 0; ok; ++wp) {
-        if (!next_piece(wp)) break;
-        const Piece& g = sh.piece[wp % kPieces];
-        wn = g.n;
-        const bool two = g.nrow > kRows;
-        if (wn == 0) break;
-#pragma unroll 1
-        for (int i = 0; ok && i < wn; ++i, ++wt) {
-          const uint32_t at = 2 * wt + 1, st = at % ST;
-          const int kk = sixteens(piece_keys(g, i, a.prefix_len, g.own));
-          const bool fresh = two ? i == 0 : i < 2, last = two ? i == wn - 1 : i >= wn - 2;
-          if (!(ok = warp_wait(sh.full + st, (at / ST) & 1, quit))) break;
-#pragma unroll 1
-          for (int sub = 0; sub <= (two ? 1 : 0); ++sub, ++s) {
-            const int l2 = s & 1;
-            if (!(ok = warp_wait(sh.p_full + l2, n_p[l2] & 1, quit))) break;
-            ++n_p[l2];
-            if (fresh) {
-              if (n_o[l2] > 0 && !(ok = warp_wait(sh.o_empty + l2, (n_o[l2] - 1) & 1, quit))) break;
-              ++n_o[l2];
-            }
-            tc::fence_after();
-            const uint64_t vd = tc::desc(ring + st * Shape::tile, kKeys * 128, 1024);
-            if (tc::elect()) {
-#pragma unroll
-              for (int j = 0; j < kKeys / 16; ++j)
-                if (j < kk)
-                  tc::mma_ts(tmem + 256 + l2 * 128, tmem + l2 * 128 + j * 8, vd + ((j * 2048) >> 4), id_o, !fresh || j > 0);
-              if (!two || sub == 1) tc::commit(sh.empty + st);
-              if (last) tc::commit(sh.o_full + l2);
-            }
-            __syncwarp();
-            if (!(ok = scores())) break;
-          }
-        }
-        done_piece(wp);
       }
-    } else if (warp < 11) {
+      __syncwarp();
+    } else if (warp == 10) {
       // --------------------------------------------------- loads of K, V ----
       // Whole pages as boxes; the rest of a tile, or a tile with a page outside
       // the pool, four rows at a time, with zeros for what is not there (a slot
@@ -883,10 +916,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
       // take are loaded.
       constexpr int PN = DP / 64;                               // 64-value panels of a row
       constexpr uint32_t kPanel = kRows * 128;
-      const int kv = warp - 9, none = (int)a.pool_rows;         // none: a row outside the map
-      const CUtensorMap *box = maps.box + kv, *one_row = maps.row + kv;
-      int32_t* rows = sh.rows[kv];
-      uint32_t pos = kv;
+      const int none = (int)a.pool_rows;                        // a row outside the map
+      int32_t* rows = sh.rows;
+      uint32_t pos = 0;
       bool ok = true;
       for (uint32_t pi = 0; ok; ++pi) {
         if (!next_piece(pi)) break;
@@ -894,9 +926,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
         const int n = g.n, x = g.kh * a.dim;
         if (n == 0) break;
 #pragma unroll 1
-        for (int i = 0; i < n; ++i, pos += 2) {
+        for (int i = 0; i < n && ok; ++i) {
           const int k0 = piece_key0(g, i) + (g.off + i < g.np ? 0 : a.prefix_len), valid = piece_keys(g, i, a.prefix_len, g.own);
-          int boxes = p.run > 0 ? valid / p.run : 0;
+          int boxes = p.run > 0 ? valid >> p.run_log : 0;
           int32_t y = 0;
           if (lane < boxes) {
             const int64_t sl = key_slot(a, g.req, k0 + lane * p.run);
@@ -916,33 +948,36 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
               }
             }
           }
-          const uint32_t st = pos % ST;
           __syncwarp();
-          if (pos >= ST && !(ok = warp_wait(sh.empty + st, (pos / ST - 1) & 1, quit))) break;
-          if (tc::elect()) {
-            uint32_t dst = ring + st * Shape::tile;
-            pipe::bar_expect_tx(sh.full + st, (uint32_t)quads * 4 * DP * 2);
 #pragma unroll 1
-            for (int b = 0; b < boxes; ++b, dst += p.run * 128) {
-              const int yb = rows[b];
+          for (int kv = 0; kv < 2; ++kv, ++pos) {
+            const uint32_t st = pos % ST;
+            if (pos >= ST && !(ok = warp_wait(sh.empty + st, (pos / ST - 1) & 1, quit))) break;
+            if (tc::elect()) {
+              uint32_t dst = ring + st * Shape::tile;
+              const CUtensorMap *box = maps.box + kv, *one_row = maps.row + kv;
+              pipe::bar_expect_tx(sh.full + st, (uint32_t)quads * 4 * DP * 2);
+#pragma unroll 2
+              for (int b = 0; b < boxes; ++b, dst += p.run * 128) {
+                const int yb = rows[b];
 #pragma unroll
-              for (int pn = 0; pn < PN; ++pn) tc::load_box(dst + pn * kPanel, box, x + pn * 64, yb, sh.full + st);
-            }
-#pragma unroll 1
-            for (int b = quad0; b < quads; ++b, dst += 512) {
-              const int4 z = *reinterpret_cast<const int4*>(rows + b * 4);
+                for (int pn = 0; pn < PN; ++pn) tc::load_box(dst + pn * kPanel, box, x + pn * 64, yb, sh.full + st);
+              }
+#pragma unroll 2
+              for (int b = quad0; b < quads; ++b, dst += 512) {
+                const int4 z = *reinterpret_cast<const int4*>(rows + b * 4);
 #pragma unroll
-              for (int pn = 0; pn < PN; ++pn) tc::load_rows(dst + pn * kPanel, one_row, x + pn * 64, z, sh.full + st);
+                for (int pn = 0; pn < PN; ++pn) tc::load_rows(dst + pn * kPanel, one_row, x + pn * 64, z, sh.full + st);
+              }
             }
+            __syncwarp();
           }
-          __syncwarp();
         }
         done_piece(pi);
       }
       // copies must not outlive the CTA: all are waited for by the products, unless a wait gave up
       if (*quit)
-        for (uint32_t q = kv; q < pos; q += 2)
-          if (q + 2 * ST >= pos) (void)pipe::bar_wait(sh.full + q % ST, (q / ST) & 1);
+        for (uint32_t q = pos > ST ? pos - ST : 0; q < pos; ++q) (void)pipe::bar_wait(sh.full + q % ST, (q / ST) & 1);
     } else {
       // ------------------------------------------ the walk, loads of Q ----
       constexpr int CH = DP / 8, RI = 32 / CH;                  // 16-byte chunks of a row; rows per instruction
@@ -998,14 +1033,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
           if (n_q >= 2 && !(ok = warp_wait(sh.q_empty + buf, ((n_q >> 1) - 1) & 1, quit))) break;
           const uint32_t dst = base + buf * Shape::tile + panel;
           const int here = nrow - b * kRows < kRows ? nrow - b * kRows : kRows;
-          const char* from = a.q + (int64_t)w.g.tok * a.q_pitch + (int64_t)(w.g.kh * a.group) * a.q_head + ch * 16;
-#pragma unroll 2
+          // row x is head x % group of token x / group; the next one of this lane's is RI further on
+          const int xs = w.g.blk * kBlock + b * kRows + sub, jt = (int)a.group_div.div((uint32_t)xs);
+          int hh = xs - jt * a.group;
+          const char* src = a.q + (int64_t)(w.g.tok + jt) * a.q_pitch + (int64_t)(w.g.kh * a.group + hh) * a.q_head + ch * 16;
+          const int64_t wrap = a.q_pitch - (int64_t)a.group * a.q_head, more = RI * a.q_head;
+#pragma unroll 4
           for (int rr = sub; rr < here; rr += RI) {
-            const int x = w.g.blk * kBlock + b * kRows + rr;
-            const int jt = (int)a.group_div.div((uint32_t)x);
-            if (in_dim)
-              tc::copy16(dst + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4),
-                         from + jt * a.q_pitch + (x - jt * a.group) * a.q_head, true);
+            if (in_dim) tc::copy16(dst + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4), src, true);
+            src += more;
+            hh += RI;
+            while (hh >= a.group) {
+              hh -= a.group;
+              src += wrap;
+            }
           }
           tc::copy_commit();
           tc::copy_wait<0>();
@@ -1019,6 +1060,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
         y = 0;
         if (left > 0) w.next();
       }
+    }
     }
   }
   // No product may be in flight when tensor memory is given back: the softmax
@@ -1178,6 +1220,9 @@ TilePlan tile_plan(const AttnArgs& a, int64_t* bytes) {
   p.ctas = sm_count();
   p.run = a.page & -a.page;  // boxes start at pages, tiles at multiples of 128 keys
   p.run = p.run < 8 ? 0 : (p.run > kKeys ? kKeys : p.run);
+  while (p.run >> (p.run_log + 1)) ++p.run_log;
+  p.slope = kBlock / (kKeys / kUnitTile) / a.group;
+  p.slope = p.slope < 1 ? 1 : p.slope;
   p.joint = a.prefix_len == 0 || a.batch == 1 || a.tokens * a.group >= (int64_t)a.batch * kRows;
   char* at = a.workspace;
   const auto take = [&](int64_t n) {
@@ -1252,6 +1297,12 @@ int launch_tiles(const AttnArgs& a, cudaStream_t s) {
   constexpr int smem = TileShape<DP>::smem;
   if (launch_cache().blocks_per_sm(attend_tile_kernel<T, DP>, kTileThreads, smem) < 0)
     return check_launch("attend_tile launch shape");
+  // a smaller launch would leave the softmax warpgroups waiting for registers that are not there
+  static const bool regs_ok = [] {
+    cudaFuncAttributes at{};
+    return cudaFuncGetAttributes(&at, attend_tile_kernel<T, DP>) == cudaSuccess && at.numRegs == kLaunchRegs;
+  }();
+  GSEC_REQUIRE(regs_ok, "attend_tile: launch registers are not %d", kLaunchRegs);
   const int rc = launch_rc(
       launch_pdl(attend_tile_kernel<T, DP>, dim3((unsigned)p.ctas), dim3(kTileThreads), smem, s, a, p, maps),
       "prefix_attention");

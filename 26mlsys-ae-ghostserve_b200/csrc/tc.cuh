@@ -152,6 +152,17 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
 // Ordinary writes to shared memory before, reads by the tensor core after.
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// The warpgroup's registers per thread from here on: more only as far as others
+// have given back of what the block was launched with.
+template <int N>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // 2^x, about 2 ulp.
 __device__ __forceinline__ float ex2(float x) {
   float y;
