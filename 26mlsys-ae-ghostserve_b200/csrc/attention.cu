@@ -183,7 +183,7 @@ int attend_rows(const AttnArgs& a, cudaStream_t s) {
 // line is one warp's work, which hands the pieces to the others through shared
 // memory, and loops are unrolled only as far as they have to be (with the walk in
 // every role and 128-column bodies a one-tile segment took 12000 cycles).
-constexpr int kTileThreads = 384;   // 2 softmax warpgroups; 2 warps issue products, 1 loads K and V, 1 walks and loads Q
+constexpr int kTileThreads = 384;   // 2 softmax warpgroups; a warp each issues products, loads K, loads V, walks and loads Q
 constexpr int kRows = 128, kKeys = 128, kBlock = 256;
 // Units of the line: a tile of a whole block; half a block's tile is three
 // quarters of that; a segment's beginning and end.
@@ -414,7 +414,10 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 template <int DP>
 struct TileShape {
   static constexpr int tile = kRows * DP * 2;                     // bytes of a Q, K or V tile
-  static constexpr int stages = DP == 128 ? 5 : 12;               // K and V tiles in flight
+  // K and V tiles in flight, a ring each: a warp that waits for a stage has seen all
+  // of its turns (a barrier tells only odd ones from even ones)
+  static constexpr uint32_t ks = DP == 128 ? 2 : 6, vs = DP == 128 ? 3 : 6;
+  static constexpr int stages = ks + vs;
   static constexpr int data = (2 + stages) * tile;
   static constexpr int smem = data + 3072;
 };
@@ -422,7 +425,7 @@ struct TileShape {
 // Shared memory behind the tiles.
 struct TileShared {
   float m[kRows], l[kRows];         // what one warpgroup hands to the other
-  alignas(16) int32_t rows[kKeys];  // pool rows of the tile being loaded
+  alignas(16) int32_t rows[2][kKeys];  // pool rows of the K and the V tile being loaded
   uint64_t full[12], empty[12], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], o_empty[2], handed, taken;
   uint64_t piece_full[kPieces], piece_empty[kPieces];
   Piece piece[kPieces];
@@ -556,18 +559,18 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const AttnArgs a, const TilePlan p,
                                                                      const __grid_constant__ PoolMaps maps) {
   using Shape = TileShape<DP>;
-  constexpr uint32_t ST = Shape::stages;
+  constexpr uint32_t KS = Shape::ks, VS = Shape::vs;
   extern __shared__ __align__(1024) unsigned char smem[];
   TileShared& sh = *reinterpret_cast<TileShared*>(smem + Shape::data);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int i = 0; i < (int)ST; ++i) {
+    for (int i = 0; i < Shape::stages; ++i) {
       pipe::bar_init(sh.full + i, 1);
-      pipe::bar_init(sh.empty + i, 2);  // both threads that issue products
+      pipe::bar_init(sh.empty + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
       pipe::bar_init(sh.q_full + i, 1);
-      pipe::bar_init(sh.q_empty + i, 2);
+      pipe::bar_init(sh.q_empty + i, 1);
       pipe::bar_init(sh.s_full + i, 1);
       pipe::bar_init(sh.p_full + i, 4);
       pipe::bar_init(sh.o_full + i, 1);
@@ -575,7 +578,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
     }
     for (int i = 0; i < kPieces; ++i) {
       pipe::bar_init(sh.piece_full + i, 1);
-      pipe::bar_init(sh.piece_empty + i, 11);  // 8 softmax warps, the loads, both threads that issue products
+      pipe::bar_init(sh.piece_empty + i, 12);  // 8 softmax warps, both loads, scores and sums of the products
     }
     pipe::bar_init(&sh.handed, 4);
     pipe::bar_init(&sh.taken, 4);
@@ -587,7 +590,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
     tc::alloc(&sh.tmem, 512);
     tc::relinquish();
   }
-  if (warp == 10 && lane < 2) {
+  if (warp == 9 && lane < 2) {
     tc::prefetch_map(maps.box + lane);
     tc::prefetch_map(maps.row + lane);
   }
@@ -810,105 +813,102 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
       }
     } else {
     tc::regs_down<kOtherRegs>();
-    if (warp < 10) {
+    if (warp == 8) {
       // -------------------------------------------------------- products ----
-      // One thread for each warpgroup's steps. A step is P V of the last and Q K^T
-      // of the next of them, whose scores take the place of that P. Issuing is slow
-      // (64 cycles a product, the rate at which they run), and so is a lone thread's
-      // arithmetic (five cycles and more an instruction): with both in one thread
-      // the tensor core waited for every other step's preparation. Here one thread
-      // prepares while the other issues.
+      // One thread. Step s runs on S, P and O number s & 1; its scores are issued
+      // right after the P V of step s - 2. A lone thread takes five cycles and more
+      // for an instruction, so the loop is kept short.
       if (tc::elect()) {
-        const int t = warp - 8;
-        const uint32_t ts = tmem + t * 128;
         const uint32_t id_s = tc::idesc(Vec16<T>::bf16, kRows, 0, false, a.scale < 0.f);
         const uint32_t id_o = tc::idesc(Vec16<T>::bf16, kRows, a.dim, true);
         const int ks = a.dim / 16;
         const uint64_t qdesc = tc::desc(base, 16, 1024), kdesc = tc::desc(ring, 16, 1024),
                        vdesc = tc::desc(ring, kKeys * 128, 1024);
-        uint32_t pi = 0, tiles = 0, n_q = 0, step = 0, n_p = 0, n_o = 0;  // pieces, tiles and Q tiles before this piece
-        int i = 0, n = 0, half = 0;
-        bool two = false;
-        // the step whose P is on its way: its V and what to do with O
-        bool have = false, fresh = false, last = false, alone = false;
-        uint32_t at = 0;
-        int kk = 0;
-        while (true) {
-          // the next step, if there is one
-          while (i >= n) {
-            if (n > 0) {
-              pipe::bar_arrive(sh.piece_empty + pi % kPieces);
-              ++pi;
-              tiles += n;
-              n_q += two ? 2 : 1;
+        uint32_t n_o0 = 0, n_o1 = 0, n_q = 0;                   // uses of the O's, Q tiles
+        // the scores' place: piece, tiles so far, tile, step of the tile; the sums' place
+        uint32_t qp = 0, qat = 0, wp = 0, wat = 0;
+        int qi = 0, qsub = 0, qn = 0, wi = 0, wsub = 0, wn = 0;
+        bool qtwo = false, wtwo = false;
+        for (uint32_t s = 0;; ++s) {                            // sums of step s - 2, scores of step s
+          const uint32_t l2 = s & 1;
+          if (s >= 2) {
+            if (wi == 0 && wsub == 0) {
+              if (!thread_wait(sh.piece_full + wp % kPieces, (wp / kPieces) & 1, quit)) break;
+              wn = sh.piece[wp % kPieces].n;
+              if (wn == 0) break;
+              wtwo = sh.piece[wp % kPieces].nrow > kRows;
             }
-            if (!thread_wait(sh.piece_full + pi % kPieces, (pi / kPieces) & 1, quit)) break;
-            const Piece& g = sh.piece[pi % kPieces];
-            n = g.n;
-            if (n == 0) break;
-            two = g.nrow > kRows;
-            half = t ^ (int)(step & 1);
-            step += two ? 2 * n : n;
-            i = two ? 0 : half;
-          }
-          if (i >= n && n > 0) break;                           // a wait gave up
-          const bool more = n > 0;
-          const Piece& g = sh.piece[pi % kPieces];
-          const int qk = more ? sixteens(piece_keys(g, i, a.prefix_len, g.own)) : 0;
-          const uint32_t q_at = 2 * (tiles + i), q_st = q_at % ST, q_buf = n_q + (two ? half : 0);
-          const uint64_t qd = qdesc + (q_buf & 1) * (Shape::tile >> 4), kd = kdesc + q_st * (Shape::tile >> 4);
-          const bool q_first = i == (two ? 0 : half), q_last = i + (two ? 1 : 2) >= n;
-          if (more) {
-            if (q_first && !thread_wait(sh.q_full + (q_buf & 1), (q_buf >> 1) & 1, quit)) break;
-            if (!thread_wait(sh.full + q_st, (q_at / ST) & 1, quit)) break;
-          }
-          if (have) {
-            const uint32_t st = at % ST;
-            const uint64_t vd = vdesc + st * (Shape::tile >> 4);
-            if (!thread_wait(sh.full + st, (at / ST) & 1, quit)) break;
-            if (fresh && n_o > 0 && !thread_wait(sh.o_empty + t, (n_o - 1) & 1, quit)) break;
-            n_o += fresh;
-            if (!thread_wait(sh.p_full + t, n_p & 1, quit)) break;
-            ++n_p;
+            const Piece& g = sh.piece[wp % kPieces];
+            const uint32_t st = KS + wat % VS;
+            const bool fresh = wi < (wtwo ? 1 : 2), last = wi >= wn - (wtwo ? 1 : 2), tile_done = !wtwo || wsub;
+            const int kk = sixteens(piece_keys(g, wi, a.prefix_len, g.own));
+            if (!thread_wait(sh.full + st, (wat / VS) & 1, quit)) break;
+            if (fresh) {
+              const uint32_t uses = l2 ? n_o1 : n_o0;
+              if (uses > 0 && !thread_wait(sh.o_empty + l2, (uses - 1) & 1, quit)) break;
+              n_o0 += l2 ^ 1;
+              n_o1 += l2;
+            }
+            if (!thread_wait(sh.p_full + l2, ((s - 2) >> 1) & 1, quit)) break;
             tc::fence_after();
-            if (kk == kKeys / 16) {
-#pragma unroll
-              for (int j = 0; j < kKeys / 16; ++j)
-                tc::mma_ts(ts + 256, ts + j * 8, vd + j * (2048 >> 4), id_o, !fresh || j > 0);
-            } else {
-#pragma unroll 1
-              for (int j = 0; j < kk; ++j) tc::mma_ts(ts + 256, ts + j * 8, vd + j * (2048 >> 4), id_o, !fresh || j > 0);
+            uint64_t vd = vdesc + st * (Shape::tile >> 4);
+            const uint32_t o = tmem + 256 + l2 * 128, pa = tmem + l2 * 128;
+#pragma unroll 4
+            for (int j = 0; j < kk; ++j, vd += 2048 >> 4) tc::mma_ts(o, pa + j * 8, vd, id_o, !fresh || j > 0);
+            if (tile_done) tc::commit(sh.empty + st);
+            if (last) tc::commit(sh.o_full + l2);
+            wsub = !tile_done;
+            if (tile_done) {
+              ++wat;
+              if (++wi == wn) {
+                wi = 0;
+                pipe::bar_arrive(sh.piece_empty + wp++ % kPieces);
+              }
             }
-            tc::commit(sh.empty + st);
-            if (alone) tc::commit(sh.empty + st);               // the other thread's arrival: it takes no part in the tile
-            if (last) tc::commit(sh.o_full + t);
           }
-          if (!more) break;
-          if (!have) tc::fence_after();
-          const uint32_t id = id_s | (uint32_t)(2 * qk) << 17;
-#pragma unroll
-          for (int j = 0; j < DP / 16; ++j) {
-            const uint32_t o = ((j >> 2) * (kRows * 128) + (j & 3) * 32) >> 4;
-            if (j < ks) tc::mma_ss(ts, qd + o, kd + o, id, j > 0);
+          if (qn < 0) continue;                                 // behind the last piece
+          if (qi == 0 && qsub == 0) {
+            if (!thread_wait(sh.piece_full + qp % kPieces, (qp / kPieces) & 1, quit)) break;
+            qn = sh.piece[qp % kPieces].n;
+            qtwo = sh.piece[qp % kPieces].nrow > kRows;
+            if (qn == 0) {
+              qn = -1;
+              continue;
+            }
           }
-          tc::commit(sh.s_full + t);
-          tc::commit(sh.empty + q_st);
-          if (!two) tc::commit(sh.empty + q_st);
-          if (q_last) {
-            tc::commit(sh.q_empty + (q_buf & 1));
-            if (two || n == 1) tc::commit(sh.q_empty + (q_buf & 1));
+          const uint32_t nq = n_q + qsub, st = qat % KS;
+          if (qi == 0 && !thread_wait(sh.q_full + (nq & 1), (nq >> 1) & 1, quit)) break;
+          if (!thread_wait(sh.full + st, (qat / KS) & 1, quit)) break;
+          tc::fence_after();
+          const Piece& g = sh.piece[qp % kPieces];
+          const uint32_t id = id_s | (uint32_t)(2 * sixteens(piece_keys(g, qi, a.prefix_len, g.own))) << 17;
+          uint64_t qd = qdesc + (nq & 1) * (Shape::tile >> 4), kd = kdesc + st * (Shape::tile >> 4);
+#pragma unroll 4
+          for (int j = 0; j < ks; ++j) {
+            tc::mma_ss(tmem + l2 * 128, qd, kd, id, j > 0);
+            const uint32_t by = (j & 3) == 3 ? (kRows * 128 - 96) >> 4 : 2;  // 32 bytes on, or to the next 64 values
+            qd += by;
+            kd += by;
           }
-          have = true;
-          fresh = q_first;
-          last = q_last;
-          alone = !two;
-          at = q_at + 1;
-          kk = qk;
-          i += two ? 1 : 2;
+          const bool tile_done = !qtwo || qsub, done = tile_done && qi == qn - 1;
+          tc::commit(sh.s_full + l2);
+          if (tile_done) tc::commit(sh.empty + st);
+          qsub = !tile_done;
+          if (tile_done) {
+            ++qat;
+            ++qi;
+          }
+          if (done) {
+            tc::commit(sh.q_empty + (n_q & 1));
+            if (qtwo) tc::commit(sh.q_empty + ((n_q + 1) & 1));
+            n_q += qtwo ? 2 : 1;
+            qi = 0;
+            pipe::bar_arrive(sh.piece_empty + qp++ % kPieces);
+          }
         }
       }
       __syncwarp();
-    } else if (warp == 10) {
+    } else if (warp < 11) {
       // --------------------------------------------------- loads of K, V ----
       // Whole pages as boxes; the rest of a tile, or a tile with a page outside
       // the pool, four rows at a time, with zeros for what is not there (a slot
@@ -916,8 +916,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
       // take are loaded.
       constexpr int PN = DP / 64;                               // 64-value panels of a row
       constexpr uint32_t kPanel = kRows * 128;
-      const int none = (int)a.pool_rows;                        // a row outside the map
-      int32_t* rows = sh.rows;
+      const int kv = warp - 9, none = (int)a.pool_rows;         // none: a row outside the map
+      const CUtensorMap *box = maps.box + kv, *one_row = maps.row + kv;
+      int32_t* rows = sh.rows[kv];
+      const uint32_t turns = kv ? VS : KS, stage0 = kv ? KS : 0;
       uint32_t pos = 0;
       bool ok = true;
       for (uint32_t pi = 0; ok; ++pi) {
@@ -926,9 +928,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
         const int n = g.n, x = g.kh * a.dim;
         if (n == 0) break;
 #pragma unroll 1
-        for (int i = 0; i < n && ok; ++i) {
+        for (int i = 0; i < n; ++i, ++pos) {
           const int k0 = piece_key0(g, i) + (g.off + i < g.np ? 0 : a.prefix_len), valid = piece_keys(g, i, a.prefix_len, g.own);
-          int boxes = p.run > 0 ? valid >> p.run_log : 0;
+          int boxes = p.run > 0 ? valid / p.run : 0;
           int32_t y = 0;
           if (lane < boxes) {
             const int64_t sl = key_slot(a, g.req, k0 + lane * p.run);
@@ -948,36 +950,33 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
               }
             }
           }
+          const uint32_t st = stage0 + pos % turns;
           __syncwarp();
+          if (pos >= turns && !(ok = warp_wait(sh.empty + st, (pos / turns - 1) & 1, quit))) break;
+          if (tc::elect()) {
+            uint32_t dst = ring + st * Shape::tile;
+            pipe::bar_expect_tx(sh.full + st, (uint32_t)quads * 4 * DP * 2);
 #pragma unroll 1
-          for (int kv = 0; kv < 2; ++kv, ++pos) {
-            const uint32_t st = pos % ST;
-            if (pos >= ST && !(ok = warp_wait(sh.empty + st, (pos / ST - 1) & 1, quit))) break;
-            if (tc::elect()) {
-              uint32_t dst = ring + st * Shape::tile;
-              const CUtensorMap *box = maps.box + kv, *one_row = maps.row + kv;
-              pipe::bar_expect_tx(sh.full + st, (uint32_t)quads * 4 * DP * 2);
-#pragma unroll 2
-              for (int b = 0; b < boxes; ++b, dst += p.run * 128) {
-                const int yb = rows[b];
+            for (int b = 0; b < boxes; ++b, dst += p.run * 128) {
+              const int yb = rows[b];
 #pragma unroll
-                for (int pn = 0; pn < PN; ++pn) tc::load_box(dst + pn * kPanel, box, x + pn * 64, yb, sh.full + st);
-              }
-#pragma unroll 2
-              for (int b = quad0; b < quads; ++b, dst += 512) {
-                const int4 z = *reinterpret_cast<const int4*>(rows + b * 4);
-#pragma unroll
-                for (int pn = 0; pn < PN; ++pn) tc::load_rows(dst + pn * kPanel, one_row, x + pn * 64, z, sh.full + st);
-              }
+              for (int pn = 0; pn < PN; ++pn) tc::load_box(dst + pn * kPanel, box, x + pn * 64, yb, sh.full + st);
             }
-            __syncwarp();
+#pragma unroll 1
+            for (int b = quad0; b < quads; ++b, dst += 512) {
+              const int4 z = *reinterpret_cast<const int4*>(rows + b * 4);
+#pragma unroll
+              for (int pn = 0; pn < PN; ++pn) tc::load_rows(dst + pn * kPanel, one_row, x + pn * 64, z, sh.full + st);
+            }
           }
+          __syncwarp();
         }
         done_piece(pi);
       }
       // copies must not outlive the CTA: all are waited for by the products, unless a wait gave up
       if (*quit)
-        for (uint32_t q = pos > ST ? pos - ST : 0; q < pos; ++q) (void)pipe::bar_wait(sh.full + q % ST, (q / ST) & 1);
+        for (uint32_t q = pos > turns ? pos - turns : 0; q < pos; ++q)
+          (void)pipe::bar_wait(sh.full + stage0 + q % turns, (q / turns) & 1);
     } else {
       // ------------------------------------------ the walk, loads of Q ----
       constexpr int CH = DP / 8, RI = 32 / CH;                  // 16-byte chunks of a row; rows per instruction
@@ -992,7 +991,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
 #pragma unroll 1
       while (true) {
         const int units = left > 0 ? w.units() : 0;
-        const int off = left > 0 ? w.tile_at(y) : 0, end = left > 0 ? w.tile_at(left < units - y ? y + left : units) : 0;
+        const int off = left > 0 && y > 0 ? w.tile_at(y) : 0;
+        const int end = left <= 0 ? 0 : (left >= units - y ? w.g.tiles : w.tile_at(y + left));
         if (left > 0 && end == off) {                           // no tile of the segment begins here
           left -= units - y;
           at += units;
@@ -1018,9 +1018,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
             g.more = w.g.len - w.g.ntok;
             g.len = w.g.len;
             g.kind = (whole && p.joint ? 1 : 0) | (end == w.g.tiles ? 2 : 0) | (whole ? 4 : 0);
-            int c0 = at / unit;                                 // the stretch in which its first tile begins
-            while (c0 < (int)blockIdx.x && w.tile_at((c0 + 1) * unit - at) == 0) ++c0;
-            g.c0 = c0;
+            if (!whole) {
+              int c0 = at / unit;                               // the stretch in which its first tile begins
+              while (c0 < (int)blockIdx.x && w.tile_at((c0 + 1) * unit - at) == 0) ++c0;
+              g.c0 = c0;
+            }
           }
         }
         __syncwarp();
@@ -1037,11 +1039,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
           const int xs = w.g.blk * kBlock + b * kRows + sub, jt = (int)a.group_div.div((uint32_t)xs);
           int hh = xs - jt * a.group;
           const char* src = a.q + (int64_t)(w.g.tok + jt) * a.q_pitch + (int64_t)(w.g.kh * a.group + hh) * a.q_head + ch * 16;
-          const int64_t wrap = a.q_pitch - (int64_t)a.group * a.q_head, more = RI * a.q_head;
+          const int64_t wrap = a.q_pitch - (int64_t)a.group * a.q_head, on_by = RI * a.q_head;
 #pragma unroll 4
           for (int rr = sub; rr < here; rr += RI) {
             if (in_dim) tc::copy16(dst + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4), src, true);
-            src += more;
+            src += on_by;
             hh += RI;
             while (hh >= a.group) {
               hh -= a.group;
