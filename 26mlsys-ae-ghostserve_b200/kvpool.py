@@ -19,14 +19,23 @@ tensors' device (or ``stream``, for which inputs must be ready); there is no CPU
 from __future__ import annotations
 
 import functools
-from dataclasses import dataclass
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
 from . import _lib, codec
 
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
+_I32 = torch.int32
+
+# A decode step makes these calls once per layer: the wrappers stay cheap (device
+# numbers instead of device objects, one allocation for several small outputs,
+# entry points looked up once).
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(name: str):
+    return getattr(_lib.lib(), name)
 
 
 def _on_stream(fn):
@@ -45,7 +54,7 @@ def _on_stream(fn):
                 raise ValueError("stream belongs to another device than the tensors")
             with torch.cuda.stream(stream):
                 return fn(*args, **kwargs)
-        if first.device.index != torch.cuda.current_device():
+        if first.get_device() != torch._C._cuda_getDevice():
             with torch.cuda.device(first.device):
                 return fn(*args, **kwargs)
         return fn(*args, **kwargs)
@@ -53,40 +62,56 @@ def _on_stream(fn):
     return call
 
 
-def _check(t, what: str, device, dtype, shape=None) -> None:
-    """A contiguous tensor of the dtype on the device, of the shape where given."""
-    if not isinstance(t, torch.Tensor) or t.device != device:
-        raise ValueError(f"{what} must be a tensor on {device}")
-    if t.dtype != dtype or not t.is_contiguous():
+def _stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _check(t, what: str, index: int, dtype, size: Optional[int] = None) -> int:
+    """A contiguous tensor of the dtype on CUDA device `index`, of `size` elements
+    where given; returns its address."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != index:
+        raise ValueError(f"{what} must be a tensor on cuda:{index}")
+    if t.dtype is not dtype or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous {dtype} tensor")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{what} must have shape {tuple(shape)}, has {tuple(t.shape)}")
+    if size is not None and t.numel() != size:
+        raise ValueError(f"{what} must have {size} elements, has {t.numel()}")
+    return t.data_ptr()
 
 
-def _check_table(table, batch: int, device) -> None:
-    if not isinstance(table, torch.Tensor) or table.device != device or table.dtype != torch.int32 or \
+def _check_out(t, shape, index: int, dtype) -> int:
+    at = _check(t, "out", index, dtype)
+    if tuple(t.shape) != shape:
+        raise ValueError(f"out must have shape {shape}, has {tuple(t.shape)}")
+    return at
+
+
+def _check_table(table, batch: int, index: int):
+    """(address, row pitch, width) of a block table."""
+    if not isinstance(table, torch.Tensor) or table.get_device() != index or table.dtype is not _I32 or \
             table.dim() != 2 or table.shape[0] != batch:
-        raise ValueError(f"table must be an int32 tensor [{batch}, pages] on {device}")
-    if table.shape[1] > 1 and table.stride(1) != 1 or batch > 1 and table.stride(0) < table.shape[1]:
+        raise ValueError(f"table must be an int32 tensor [{batch}, pages] on cuda:{index}")
+    width = table.shape[1]
+    pitch, one = table.stride()
+    if width > 1 and one != 1 or batch > 1 and pitch < width:
         raise ValueError("the rows of table must be contiguous and must not overlap")
+    return table.data_ptr(), (pitch if pitch > width else width), width
 
 
-def _pool_record(pool, device, dtype):
-    """(slot pitch, V plane offset) in bytes of a pool [slots, 2, heads, dim]."""
+def _pool_record(pool, index: int, dtype):
+    """(heads, dim, slot pitch, V plane offset) of a pool [slots, 2, heads, dim], the last two in bytes."""
     if not isinstance(pool, torch.Tensor) or pool.dim() != 4 or pool.shape[1] != 2:
         raise ValueError("pool must be a CUDA tensor [slots, 2 (K, V), heads, dim]")
-    if pool.device != device or pool.dtype != dtype:
-        raise ValueError(f"pool must be a {dtype} tensor on {device}")
-    h, d = pool.shape[2], pool.shape[3]
-    s = pool.stride()
-    if (d > 1 and s[3] != 1) or (h > 1 and s[2] != d):
+    if pool.get_device() != index or pool.dtype is not dtype:
+        raise ValueError(f"pool must be a {dtype} tensor on cuda:{index}")
+    _, _, h, d = pool.shape
+    pitch, plane, head, one = pool.stride()
+    if (d > 1 and one != 1) or (h > 1 and head != d):
         raise ValueError("a pool row (pool[slot, plane]) must be contiguous")
     es = pool.element_size()
-    return s[0] * es, s[1] * es
+    return h, d, pitch * es, plane * es
 
 
-@dataclass(frozen=True)
-class SlotPlan:
+class SlotPlan(NamedTuple):
     """Where a batch's new tokens go: one slot and position per token, request by
     request, padded with slot -1 and position 0."""
     slots: torch.Tensor       # int64 [tokens]
@@ -110,26 +135,24 @@ def slots_plan(lens: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free:
     position (the length of a shared prefix). Too few free pages, a row longer
     than the table, more tokens than ``tokens`` or a negative length give slot -1
     where a token has no place, and set bit 17 of ``codec.device_status``."""
-    dev = lens.device
-    batch = lens.numel()
-    _check(lens, "lens", dev, torch.int32, (batch,))
-    _check(new, "new", dev, torch.int32, (batch,))
-    _check_table(table, batch, dev)
-    _check(free, "free", dev, torch.int32, (free.numel(),) if isinstance(free, torch.Tensor) else None)
-    _check(cursor, "cursor", dev, torch.int32, (1,))
+    index, batch = lens.get_device(), lens.numel()
+    if lens.dim() != 1:
+        raise ValueError("lens must have one dimension")
+    lens_at = _check(lens, "lens", index, _I32)
+    new_at = _check(new, "new", index, _I32, batch)
+    table_at, pitch, width = _check_table(table, batch, index)
+    free_at = _check(free, "free", index, _I32)
+    cursor_at = _check(cursor, "cursor", index, _I32, 1)
     tokens = int(tokens)
     if tokens < 0:
         raise ValueError("tokens must not be negative")
-    slots = torch.empty(tokens, dtype=torch.int64, device=dev)
-    # the four int32 outputs share one allocation; positions first, so that it is aligned
-    n = -(-tokens // 4) * 4
-    small = torch.empty(n + 2 * batch + 2, dtype=torch.int32, device=dev)
-    positions, cu = small[:tokens], small[n:n + batch + 1]
-    out, taken = small[n + batch + 1:n + 2 * batch + 1], small[n + 2 * batch + 1:]
-    _lib.call("gsec_slots_plan", lens.data_ptr(), new.data_ptr(), batch, table.data_ptr(),
-              max(table.stride(0), table.shape[1]), table.shape[1], free.data_ptr(), free.numel(), cursor.data_ptr(),
-              int(page), int(base), slots.data_ptr(), positions.data_ptr(), tokens, cu.data_ptr(), out.data_ptr(),
-              taken.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    slots = torch.empty(tokens, dtype=torch.int64, device=lens.device)
+    # the int32 outputs share one allocation, the per-token one in front
+    positions, cu, out, taken = lens.new_empty(tokens + 2 * batch + 2).split_with_sizes((tokens, batch + 1, batch, 1))
+    _lib.check(_entry("gsec_slots_plan")(
+        lens_at, new_at, batch, table_at, pitch, width, free_at, free.numel(), cursor_at, int(page), int(base),
+        slots.data_ptr(), positions.data_ptr(), tokens, cu.data_ptr(), out.data_ptr(), taken.data_ptr(),
+        _stream(index)))
     return SlotPlan(slots, positions, cu, out, taken, table, int(page))
 
 
@@ -150,39 +173,39 @@ def qk_norm_rope_store(qkv: torch.Tensor, pool: torch.Tensor, slots: torch.Tenso
     rounding. A slot past the pool stores nothing and sets bit 16 of
     ``codec.device_status``; a position outside the tables leaves the row
     unrotated and sets bit 18."""
-    dev, dt = qkv.device, qkv.dtype
+    index, dt = qkv.get_device(), qkv.dtype
     if dt not in _DTYPES or qkv.dim() != 2 or qkv.shape[1] > 1 and qkv.stride(1) != 1:
         raise ValueError("qkv must be a bf16, fp16 or fp32 tensor [tokens, values] with contiguous rows")
-    pitch, plane = _pool_record(pool, dev, dt)
-    T, hk, D = qkv.shape[0], pool.shape[2], pool.shape[3]
+    hk, D, pitch, plane = _pool_record(pool, index, dt)
+    T, values = qkv.shape
     heads = int(heads)
-    if qkv.shape[1] != (heads + 2 * hk) * D:
-        raise ValueError(f"qkv rows hold {qkv.shape[1]} values, {heads} + 2*{hk} heads of {D} need "
-                         f"{(heads + 2 * hk) * D}")
-    codec._slot_list(slots, dev)
+    if values != (heads + 2 * hk) * D:
+        raise ValueError(f"qkv rows hold {values} values, {heads} + 2*{hk} heads of {D} need {(heads + 2 * hk) * D}")
+    codec._slot_list(slots, qkv.device)
     if slots.numel() != T:
         raise ValueError(f"slots has {slots.numel()} entries for {T} tokens")
-    if not isinstance(positions, torch.Tensor) or positions.device != dev or \
-            positions.dtype not in (torch.int32, torch.int64) or not positions.is_contiguous() or \
-            positions.numel() != T:
-        raise ValueError(f"positions must be a contiguous int32 or int64 tensor of {T} entries on {dev}")
-    _check(cos, "cos", dev, torch.float32)
+    if not isinstance(positions, torch.Tensor) or positions.get_device() != index or \
+            positions.dtype not in (_I32, torch.int64) or not positions.is_contiguous() or positions.numel() != T:
+        raise ValueError(f"positions must be a contiguous int32 or int64 tensor of {T} entries on cuda:{index}")
+    cos_at = _check(cos, "cos", index, torch.float32)
     if cos.dim() != 2:
         raise ValueError("cos must have shape [positions, rot / 2]")
-    _check(sin, "sin", dev, torch.float32, cos.shape)
-    for w, what in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if w is not None:
-            _check(w, what, dev, dt, (D,))
+    sin_at = _check(sin, "sin", index, torch.float32)
+    if sin.shape != cos.shape:
+        raise ValueError(f"sin must have the shape of cos, {tuple(cos.shape)}")
+    qw = None if q_weight is None else _check(q_weight, "q_weight", index, dt, D)
+    kw = None if k_weight is None else _check(k_weight, "k_weight", index, dt, D)
     if out is None:
-        out = torch.empty(T, heads, D, dtype=dt, device=dev)
+        out = torch.empty((T, heads, D), dtype=dt, device=qkv.device)
+        out_at = out.data_ptr()
     else:
-        _check(out, "out", dev, dt, (T, heads, D))
-    _lib.call("gsec_qk_norm_rope_store", qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1]) * qkv.element_size(), T,
-              _DTYPES[dt], heads, hk, D, out.data_ptr(), pool.data_ptr(), pitch, plane, pool.shape[0],
-              slots.data_ptr(), slots.element_size(), positions.data_ptr(), positions.element_size(), cos.data_ptr(),
-              sin.data_ptr(), 2 * cos.shape[1], cos.shape[0], None if q_weight is None else q_weight.data_ptr(),
-              None if k_weight is None else k_weight.data_ptr(), float(eps), int(bool(interleaved)),
-              torch.cuda.current_stream().cuda_stream)
+        out_at = _check_out(out, (T, heads, D), index, dt)
+    row = qkv.stride(0)
+    _lib.check(_entry("gsec_qk_norm_rope_store")(
+        qkv.data_ptr(), (row if row > values else values) * qkv.element_size(), T, _DTYPES[dt], heads, hk, D, out_at,
+        pool.data_ptr(), pitch, plane, pool.shape[0], slots.data_ptr(), slots.element_size(), positions.data_ptr(),
+        positions.element_size(), cos_at, sin_at, 2 * cos.shape[1], cos.shape[0], qw, kw, float(eps),
+        int(bool(interleaved)), _stream(index)))
     return out
 
 
@@ -203,45 +226,49 @@ def prefix_attention(q: torch.Tensor, pool: torch.Tensor, cu: torch.Tensor, lens
     non-finite value may spread to earlier tokens of the same request); slots outside
     all lengths may hold anything. A page outside the pool reads as zeros and a
     length past the table is cut; both set bit 19 of ``codec.device_status``."""
-    dev, dt = q.device, q.dtype
+    index, dt = q.get_device(), q.dtype
     if dt not in _DTYPES or q.dim() != 3 or q.shape[2] > 1 and q.stride(2) != 1:
         raise ValueError("q must be a bf16, fp16 or fp32 tensor [tokens, heads, dim] with contiguous heads")
-    pitch, plane = _pool_record(pool, dev, dt)
+    hk, d, pitch, plane = _pool_record(pool, index, dt)
     T, hq, D = q.shape
-    hk = pool.shape[2]
-    if pool.shape[3] != D or hk == 0 or hq % hk:
-        raise ValueError(f"pool heads {tuple(pool.shape[2:])} do not serve queries {tuple(q.shape[1:])}")
-    batch = lens.numel() if isinstance(lens, torch.Tensor) else -1
-    _check(lens, "lens", dev, torch.int32, (batch,))
-    _check(cu, "cu", dev, torch.int32, (batch + 1,))
-    _check_table(table, batch, dev)
+    if d != D or hk == 0 or hq % hk:
+        raise ValueError(f"pool heads {(hk, d)} do not serve queries {(hq, D)}")
+    lens_at = _check(lens, "lens", index, _I32)
+    batch = lens.numel()
+    cu_at = _check(cu, "cu", index, _I32, batch + 1)
+    table_at, row, width = _check_table(table, batch, index)
     page, prefix_len = int(page), int(prefix_len)
     if prefix_len < 0 or page < 1:
         raise ValueError("prefix_len must not be negative, page must be positive")
+    prefix_at = None
     if prefix_len:
         if prefix is None:
             raise ValueError("prefix_len without prefix pages")
-        _check(prefix, "prefix", dev, torch.int32)
+        prefix_at = _check(prefix, "prefix", index, _I32)
         if prefix.numel() * page < prefix_len:
             raise ValueError(f"{prefix.numel()} prefix pages of {page} hold fewer than {prefix_len} keys")
     if out is None:
-        out = torch.empty(T, hq, D, dtype=dt, device=dev)
+        out = torch.empty((T, hq, D), dtype=dt, device=q.device)
+        out_at = out.data_ptr()
     else:
-        _check(out, "out", dev, dt, (T, hq, D))
-    lse = torch.empty(T, hq, dtype=torch.float32, device=dev) if return_lse else None
-    nbytes = _workspace_bytes(T, batch, prefix_len, _DTYPES[dt], hq, hk, D)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        out_at = _check_out(out, (T, hq, D), index, dt)
+    lse = torch.empty((T, hq), dtype=torch.float32, device=q.device) if return_lse else None
+    code = _DTYPES[dt]
+    nbytes = _workspace_bytes(index, T, batch, prefix_len, code, hq, hk, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     es = q.element_size()
-    _lib.call("gsec_prefix_attention", q.data_ptr(), q.stride(0) * es, q.stride(1) * es, T, _DTYPES[dt], hq, hk, D,
-              pool.data_ptr(), pitch, plane, pool.shape[0], cu.data_ptr(), lens.data_ptr(), batch, table.data_ptr(),
-              max(table.stride(0), table.shape[1]), table.shape[1], page, prefix.data_ptr() if prefix_len else None,
-              prefix_len, D ** -0.5 if scale is None else float(scale), out.data_ptr(),
-              lse.data_ptr() if return_lse else None, ws.data_ptr() if nbytes else None, nbytes,
-              torch.cuda.current_stream().cuda_stream)
+    q_row, q_head, _ = q.stride()
+    _lib.check(_entry("gsec_prefix_attention")(
+        q.data_ptr(), q_row * es, q_head * es, T, code, hq, hk, D, pool.data_ptr(), pitch, plane, pool.shape[0],
+        cu_at, lens_at, batch, table_at, row, width, page, prefix_at, prefix_len,
+        D ** -0.5 if scale is None else float(scale), out_at, lse.data_ptr() if return_lse else None,
+        ws.data_ptr() if nbytes else None, nbytes, _stream(index)))
     return (out, lse) if return_lse else out
 
 
-def _workspace_bytes(tokens, batch, prefix_len, dtype, hq, hk, dim) -> int:
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(index, tokens, batch, prefix_len, dtype, hq, hk, dim) -> int:
+    """Asked once per shape and device (its size goes by the number of SMs)."""
     out = _lib.C.c_int64(0)
     _lib.call("gsec_prefix_attention_workspace", tokens, batch, prefix_len, dtype, hq, hk, dim, _lib.C.byref(out))
     return int(out.value)
