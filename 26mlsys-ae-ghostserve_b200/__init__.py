@@ -14,6 +14,9 @@ benchmark   drop-ins for the reference's benchmark/{xor,rdp,rs}/main.py
 hook        drop-in for the reference's SGLang forward_extend KV hook
 p2p         CUDA-IPC peer mapping of KV buffers across the ranks of a node
 offload     pinned-host parity ring: pipelined device<->host encode and restore
+kvpool      serving a paged KV pool: slot plans, norm / rotation / store of new tokens,
+            attention with a shared prefix
+prefill     tensor-parallel prefill and ragged extend steps that drive the hook
 """
 from . import _lib  # noqa: F401
 from .codec import CodeSpec, decode, encode, parity_bytes  # noqa: F401

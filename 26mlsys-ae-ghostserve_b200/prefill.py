@@ -19,6 +19,12 @@ KV cache layout: SGLang's FlashInfer pool, one pool per layer of
 default; slot = token position), or a layer-major ``[layers, kv_heads_rank,
 max_tokens, 128]`` pair (``layout="layer"``).
 
+Attention: torch's (``attention="sdpa"``, the default, any device), or this
+package's KV-pool operators (``attention="pool"``, CUDA, layout "pool"): queries
+and keys are normed, rotated and stored in one pass and attention reads the pool
+in place. ``TPPrefill.extend`` runs a ragged batch with them: requests of any
+lengths on pages of the pool, decode steps among them, behind a shared prefix.
+
 Parity variants (``run_prefill``):
 * ``"hook"``: the drop-in hook as SGLang drives it — a FlashInfer-named
   attention backend patched with ``hook.patch_backend``; after every layer's
@@ -45,6 +51,8 @@ import torch.distributed as dist
 import torch.nn.functional as F
 from torch.nn.attention.bias import causal_lower_right
 
+from . import kvpool
+
 
 @dataclass(frozen=True)
 class ModelSpec:
@@ -57,12 +65,14 @@ class ModelSpec:
     vocab: int = 128256
     rope_theta: float = 500000.0
     eps: float = 1e-5
+    qk_norm: bool = False  # root-mean-square norm of every query and key head before the rotation
 
 
 class TPPrefill:
     """One rank's slice of the model and its KV cache."""
 
-    def __init__(self, spec: ModelSpec, max_tokens: int, device, group=None, seed: int = 0, layout: str = "pool"):
+    def __init__(self, spec: ModelSpec, max_tokens: int, device, group=None, seed: int = 0, layout: str = "pool",
+                 attention: str = "sdpa"):
         self.spec = spec
         self.group = group
         self.world = dist.get_world_size(group) if dist.is_initialized() else 1
@@ -84,11 +94,17 @@ class TPPrefill:
                 wqkv=rnd(H, (self.hq + 2 * self.hk) * D), wo=rnd(self.hq * D, H),
                 w13=rnd(H, 2 * self.f), w2=rnd(self.f, H),
                 ln1=torch.ones(H, device=self.device, dtype=torch.bfloat16),
-                ln2=torch.ones(H, device=self.device, dtype=torch.bfloat16)))
+                ln2=torch.ones(H, device=self.device, dtype=torch.bfloat16),
+                qn=torch.ones(D, device=self.device, dtype=torch.bfloat16) if spec.qk_norm else None,
+                kn=torch.ones(D, device=self.device, dtype=torch.bfloat16) if spec.qk_norm else None))
         self.embed = rnd(spec.vocab, H, std=1.0)
         if layout not in ("pool", "layer"):
             raise ValueError("layout must be 'pool' or 'layer'")
-        self.layout = layout
+        if attention not in ("sdpa", "pool"):
+            raise ValueError("attention must be 'sdpa' or 'pool'")
+        if attention == "pool" and (layout != "pool" or self.device.type != "cuda"):
+            raise ValueError("attention 'pool' needs layout 'pool' on a CUDA device")
+        self.layout, self.attention = layout, attention
         if layout == "pool":  # per layer [slots, 2, kv_heads, D]: slot s holds token s's K and V
             self.pool = torch.empty(spec.layers, max_tokens, 2, self.hk, D, device=self.device, dtype=torch.bfloat16)
         else:
@@ -98,6 +114,10 @@ class TPPrefill:
         ang = torch.outer(torch.arange(max_tokens, device=self.device, dtype=torch.float32), inv)
         self.cos, self.sin = ang.cos(), ang.sin()
         self.max_tokens = max_tokens
+
+        if attention == "pool":  # forward_chunk's one request: slot = token position, in pages as large as fit
+            self._page = next(n for n in (128, 64, 32, 16, 8, 4, 2, 1) if max_tokens % n == 0)
+            self._table = torch.arange(max_tokens // self._page, device=self.device, dtype=torch.int32)[None]
 
     def _norm(self, x, w):
         xf = x.float()
@@ -122,14 +142,26 @@ class TPPrefill:
         T = ids.numel()
         if pos0 + T > self.max_tokens:
             raise ValueError("chunk past the end of the KV cache")
+        if self.attention == "pool":
+            lens = torch.tensor([0, T, pos0 + T], device=self.device, dtype=torch.int32)
+            at = torch.arange(pos0, pos0 + T, device=self.device)
+            plan = kvpool.SlotPlan(at, at.int(), lens[:2], lens[2:], None, self._table, self._page)
+            after = None
+            if after_attention is not None:
+                def after(li):
+                    now = self.pool[li, pos0:pos0 + T]
+                    after_attention(li, now[:, 0].transpose(0, 1), now[:, 1].transpose(0, 1))
+            return self._extend(ids, plan, None, 0, after)
         D, hq, hk = self.spec.head_dim, self.hq, self.hk
         x = self.embed[ids]
         mask = causal_lower_right(T, pos0 + T)
         for li, L in enumerate(self.layers):
             h = self._norm(x, L["ln1"])
             qkv = h @ L["wqkv"]
-            q = self._rope(qkv[:, :hq * D].view(T, hq, D), pos0)
-            k = self._rope(qkv[:, hq * D:(hq + hk) * D].view(T, hk, D), pos0)
+            q, k = qkv[:, :hq * D].view(T, hq, D), qkv[:, hq * D:(hq + hk) * D].view(T, hk, D)
+            if self.spec.qk_norm:
+                q, k = self._norm(q, L["qn"]), self._norm(k, L["kn"])
+            q, k = self._rope(q, pos0), self._rope(k, pos0)
             v = qkv[:, (hq + hk) * D:].view(T, hk, D)
             if self.layout == "pool":
                 self.pool[li, pos0:pos0 + T, 0] = k
@@ -144,12 +176,43 @@ class TPPrefill:
                                                enable_gqa=hq != hk)
             if after_attention is not None:
                 after_attention(li, kc[:, pos0:pos0 + T], vc[:, pos0:pos0 + T])
-            o = o[0].transpose(0, 1).reshape(T, hq * D) @ L["wo"]
-            x = x + self._all_reduce(o)
-            h = self._norm(x, L["ln2"])
-            gu = h @ L["w13"]
-            a = F.silu(gu[:, :self.f]) * gu[:, self.f:]
-            x = x + self._all_reduce(a @ L["w2"])
+            x = self._after_attention(x, o[0].transpose(0, 1).reshape(T, hq * D), L)
+        return x
+
+    def _after_attention(self, x, o, L):
+        """The rest of a layer: output projection and the feed-forward part."""
+        x = x + self._all_reduce(o @ L["wo"])
+        gu = self._norm(x, L["ln2"]) @ L["w13"]
+        a = F.silu(gu[:, :self.f]) * gu[:, self.f:]
+        return x + self._all_reduce(a @ L["w2"])
+
+    def extend(self, ids: torch.Tensor, plan: kvpool.SlotPlan, prefix: Optional[torch.Tensor] = None,
+               prefix_len: int = 0, after_attention: Optional[Callable[[int], None]] = None) -> torch.Tensor:
+        """Run a ragged batch's new tokens through every layer; returns [tokens, hidden].
+
+        ``ids`` are the new tokens request by request, ``plan`` where they go
+        (``kvpool.slots_plan``, with ``base=prefix_len`` when the batch shares the
+        ``prefix_len`` tokens on the pages ``prefix``, already in the pool). One new
+        token per request is a decode step. Rows behind the last request (a batch
+        padded for a captured graph) are computed but mean nothing.
+        ``after_attention(li)`` is called after each layer's attention, when the
+        plan's slots of ``layer_pool(li)`` hold the new keys and values."""
+        if self.attention != "pool":
+            raise ValueError("extend needs attention='pool'")
+        return self._extend(ids, plan, prefix, prefix_len, after_attention)
+
+    def _extend(self, ids, plan, prefix, prefix_len, after_attention):
+        T, D = ids.numel(), self.spec.head_dim
+        x = self.embed[ids]
+        for li, L in enumerate(self.layers):
+            qkv = self._norm(x, L["ln1"]) @ L["wqkv"]
+            q = kvpool.qk_norm_rope_store(qkv, self.pool[li], plan.slots, plan.positions, self.cos, self.sin, self.hq,
+                                          q_weight=L["qn"], k_weight=L["kn"], eps=self.spec.eps)
+            o = kvpool.prefix_attention(q, self.pool[li], plan.cu, plan.lens, plan.table, plan.page, prefix=prefix,
+                                        prefix_len=prefix_len)
+            if after_attention is not None:
+                after_attention(li)
+            x = self._after_attention(x, o.view(T, self.hq * D), L)
         return x
 
     def chunk_kv_parts(self, pos0: int, T: int):

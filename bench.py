@@ -246,6 +246,8 @@ def main():
     ap.add_argument("--prefill-len", type=int, default=32768)
     ap.add_argument("--prefill-chunk", type=int, default=2048)
     ap.add_argument("--prefill-layers", type=int, default=32)
+    ap.add_argument("--prefill-attention", default="sdpa", choices=["sdpa", "pool"],
+                    help="prefill workload: torch's attention, or this package's KV-pool operators")
     ap.add_argument("--parity", default="none,hook_chunk,hook,reference",
                     help="prefill variants to time: none; hook (the drop-in hook on every layer's "
                          "forward_extend, one encode per call, as SGLang drives the reference hook); hook_chunk (the "
@@ -1060,7 +1062,7 @@ def run_prefill_bench(args):
     pre = importlib.import_module(PKG + ".prefill")
     hook = importlib.import_module(PKG + ".hook")
     spec = pre.ModelSpec(layers=args.prefill_layers)
-    model = pre.TPPrefill(spec, args.prefill_len, device)
+    model = pre.TPPrefill(spec, args.prefill_len, device, attention=args.prefill_attention)
     chunk = args.prefill_chunk
     variants = [v for v in args.parity.split(",") if v]
     rates, times, recovery = {}, {}, {}
@@ -1101,6 +1103,7 @@ def run_prefill_bench(args):
             "scaling": "strong", "dtype": "bf16", "data": "synthetic (uniform random token ids)",
             "config": {"workload": "prefill", "tp": world, "seqs": args.prefill_seqs, "seq_len": args.prefill_len,
                        "chunk": chunk, "layers": args.prefill_layers, "value_variant": head,
+                       "attention": args.prefill_attention,
                        "kv_cache": "per-layer pools [slots, 2, kv_heads/TP, 128] bf16 (SGLang FlashInfer layout)",
                        "parity_code": "hook/hook_chunk/fused: RDP over the TP ranks' delta KV (k = TP), "
                                       "reference: mod-S RDP gathered to a rotating rank per layer call",

@@ -70,3 +70,31 @@ def test_hook_variant_calls_forward_extend_per_layer():
     assert [s[0] for s in seen] == [0, 1, 2, 0, 1, 2]
     assert [s[1] for s in seen[:3]] == [m.layer_pool(li).data_ptr() for li in range(3)]
     assert seen[0][2] == list(range(8)) and seen[3][2] == list(range(8, 16))
+
+
+def test_qk_norm_prefill_equals_one_shot():
+    pre = pkg("prefill")
+    spec = pre.ModelSpec(**SPEC, qk_norm=True)
+    ids = torch.randint(0, 50, (32,), generator=torch.Generator().manual_seed(5))
+    one, chunked = pre.TPPrefill(spec, 32, "cpu"), pre.TPPrefill(spec, 32, "cpu")
+    one.forward_chunk(ids, 0)
+    for i in range(0, 32, 8):
+        chunked.forward_chunk(ids[i:i + 8], i)
+    # a product's sums may run in another order for another number of rows: the same values up to bf16 roundings
+    # (half a step, 2^-8), ten to a layer, on two layers and two sides
+    a, b = one.pool.double(), chunked.pool.double()
+    assert float((a - b).norm() / a.norm()) <= 2 * 2 * 10 * 2.0 ** -8
+    plain = pre.TPPrefill(pre.ModelSpec(**SPEC), 32, "cpu")
+    plain.forward_chunk(ids, 0)
+    assert not torch.equal(plain.pool[:, :, 0], one.pool[:, :, 0])
+
+
+def test_pool_attention_is_refused_where_it_cannot_run():
+    pre = pkg("prefill")
+    spec = pre.ModelSpec(**SPEC)
+    with pytest.raises(ValueError, match="CUDA"):
+        pre.TPPrefill(spec, 32, "cpu", attention="pool")
+    with pytest.raises(ValueError, match="attention"):
+        pre.TPPrefill(spec, 32, "cpu", attention="flash")
+    with pytest.raises(ValueError, match="pool"):
+        pre.TPPrefill(spec, 32, "cpu").extend(torch.arange(4), None)
