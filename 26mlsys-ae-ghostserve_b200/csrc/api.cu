@@ -636,8 +636,8 @@ int gsec_qk_norm_rope_store(const void* qkv, int64_t qkv_pitch, int64_t tokens, 
                rot);
   GSEC_REQUIRE(max_pos >= 0 && (rot == 0 || (cos && sin)), "null pointer (cos, sin)");
   GSEC_REQUIRE(aligned16(qkv) && (qkv_pitch & 15) == 0 && aligned16(q_out) && aligned16(q_weight) &&
-                   aligned16(k_weight),
-               "qkv, its pitch, q_out and the weights must be 16-byte aligned");
+                   aligned16(k_weight) && aligned16(cos) && aligned16(sin),
+               "qkv, its pitch, q_out, cos, sin and the weights must be 16-byte aligned");
   GSEC_REQUIRE(qkv_pitch >= (int64_t)(hq + 2 * hk) * dim * es, "qkv rows overlap");
   QkStoreArgs a{};
   a.qkv = static_cast<const char*>(qkv);
@@ -661,7 +661,9 @@ int gsec_qk_norm_rope_store(const void* qkv, int64_t qkv_pitch, int64_t tokens, 
   a.k_weight = k_weight;
   a.eps = eps;
   a.interleaved = interleaved != 0;
-  return qk_norm_rope_store(a, dtype, slot_bytes, position_bytes, as_stream(stream));
+  a.slot_bytes = slot_bytes;
+  a.position_bytes = position_bytes;
+  return qk_norm_rope_store(a, dtype, as_stream(stream));
 }
 
 int gsec_prefix_attention_workspace(int64_t tokens, int32_t batch, int64_t prefix_len, int32_t dtype, int32_t hq,

@@ -169,155 +169,199 @@ __global__ void __launch_bounds__(kPlanThreads) slots_plan_kernel(const SlotPlan
 // rounded once at the store.
 //
 // A head is a group of G lanes (a power of two >= dim / vector), one 16-byte
-// vector per lane: the sum of squares and the partner values of the rotation
+// vector per lane: the sum of squares and the partner vectors of the rotation
 // move by shuffles, and every load and store is one coalesced vector. A group
-// takes H consecutive heads of one token, so that a token's cos and sin rows
-// are read once per H heads and H loads are in flight per lane.
+// takes up to H heads of one kind (query, key, value) of one token, so that a
+// token's cos and sin rows are read once per H heads and H loads are in flight
+// per lane. With the weights folded into cos and sin a head is
+// r (x (w c) + y (w' s)), y the partner's values as they came: one shuffle per
+// word of two values, before they are unpacked.
 constexpr int kStoreThreads = 256;
+constexpr int kStoreHeads = 4;
 
-template <typename T, typename SI, typename PI, int H>
-__global__ void __launch_bounds__(kStoreThreads) qk_store_kernel(const QkStoreArgs a, int G) {
-  using V = Vec16<T>;
-  grid_dep_wait();
-  grid_dep_launch();
-  const int heads = a.hq + 2 * a.hk;
-  const int parts = (heads + H - 1) / H;
-  const int64_t groups = a.tokens * parts;
-  const int lane = threadIdx.x % G;              // lane in its group
-  const int vecs = a.dim / V::N, half = a.rot / 2;
-  const bool live = lane < vecs;
-  const bool turns = lane * V::N < a.rot;
-  // partner lane of the split-half rotation; its sign
-  const int hv = half / V::N;
-  const int partner = a.interleaved || !turns ? lane : (lane < hv ? lane + hv : lane - hv);
-  const float sign = lane < hv ? -1.f : 1.f;
-  const int64_t step = (int64_t)gridDim.x * (kStoreThreads / G);
-  const int64_t g0 = (int64_t)blockIdx.x * (kStoreThreads / G) + threadIdx.x / G;
-  const int64_t rounds = (groups + step - 1) / step;  // the same for every lane: shuffles stay whole
-  for (int64_t it = 0; it < rounds; ++it) {
-    const int64_t g = g0 + it * step;
-    const bool on = g < groups;
-    const int64_t t = on ? g / parts : 0;
-    const int h0 = on ? (int)(g - t * parts) * H : 0;
-    const char* row = a.qkv + t * a.qkv_pitch + (int64_t)lane * 16;
-    uint4 raw[H];
+// Four values of a cos or sin row (two for 32-bit pairs of neighbours).
+template <int N>
+__device__ __forceinline__ void load_angles(const float* at, float* f) {
+  if (N == 2) {
+    const float2 v = __ldg(reinterpret_cast<const float2*>(at));
+    f[0] = v.x;
+    f[1] = v.y;
+  } else {
 #pragma unroll
-    for (int j = 0; j < H; ++j)
-      if (on && live && h0 + j < heads)
-        raw[j] = __ldg(reinterpret_cast<const uint4*>(row + (int64_t)(h0 + j) * a.dim * sizeof(T)));
-      else
-        raw[j] = vzero();
-    float c[V::N], s[V::N];
-    if (on && h0 < a.hq + a.hk) {
-      const int64_t pos = (int64_t)static_cast<const PI*>(a.positions)[t];
-      const bool in = pos >= 0 && pos < a.max_pos;
-      if (!in && lane == 0) atomicOr(&g_kvpool_status, 4u);
-      if (in && live && turns) {
-        const float* cr = a.cos + pos * half;
-        const float* sr = a.sin + pos * half;
-        if (a.interleaved) {
-#pragma unroll
-          for (int e = 0; e < V::N; ++e) {
-            c[e] = __ldg(cr + (lane * V::N + e) / 2);
-            s[e] = __ldg(sr + (lane * V::N + e) / 2) * (e & 1 ? 1.f : -1.f);
-          }
-        } else {
-          const int at = (lane < hv ? lane : lane - hv) * V::N;
-#pragma unroll
-          for (int e = 0; e < V::N; ++e) {
-            c[e] = __ldg(cr + at + e);
-            s[e] = __ldg(sr + at + e) * sign;
-          }
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < V::N; ++e) {
-          c[e] = 1.f;
-          s[e] = 0.f;
-        }
-      }
-    }
-    int64_t slot = -1;
-    if (on && h0 + H > a.hq) {
-      slot = (int64_t)static_cast<const SI*>(a.slots)[t];
-      if (slot >= a.pool_rows) {
-        if (lane == 0) atomicOr(&g_kvpool_status, 1u);
-        slot = -1;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < H; ++j) {
-      const int h = h0 + j;
-      uint4 res = raw[j];
-      const bool qk = on && h < a.hq + a.hk;
-      float x[V::N];
-      V::unpack(raw[j], x);
-      const void* w = h < a.hq ? a.q_weight : a.k_weight;
-      if (a.q_weight != nullptr || a.k_weight != nullptr) {  // the same for every lane
-        float ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < V::N; ++e) ss += x[e] * x[e];
-        for (int d = G >> 1; d; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-        float down = 1.f;
-        if (__any_sync(0xffffffffu, ss == INFINITY)) {  // squares past 32 bits: the same with x 2^-64
-          float st = 0.f;
-#pragma unroll
-          for (int e = 0; e < V::N; ++e) st += (x[e] * 0x1p-64f) * (x[e] * 0x1p-64f);
-          for (int d = G >> 1; d; d >>= 1) st += __shfl_xor_sync(0xffffffffu, st, d);
-          if (ss == INFINITY) {
-            ss = st;
-            down = 0x1p-64f;
-          }
-        }
-        if (qk && live && w != nullptr) {
-          const float r = 1.f / sqrtf(ss / (float)a.dim + a.eps * down * down);
-          float wf[V::N];
-          V::unpack(__ldg(reinterpret_cast<const uint4*>(w) + lane), wf);
-#pragma unroll
-          for (int e = 0; e < V::N; ++e) x[e] = x[e] * down * r * wf[e];
-        }
-      }
-      float y[V::N];
-#pragma unroll
-      for (int e = 0; e < V::N; ++e)
-        y[e] = a.interleaved ? x[e ^ 1] : __shfl_sync(0xffffffffu, x[e], partner, G);
-      if (qk && turns) {
-#pragma unroll
-        for (int e = 0; e < V::N; ++e) x[e] = x[e] * c[e] + y[e] * s[e];
-      }
-      if (qk) res = V::pack(x);
-      if (!on || !live || h >= heads) continue;
-      if (h < a.hq) {
-        *reinterpret_cast<uint4*>(a.q_out + ((t * a.hq + h) * a.dim) * (int64_t)sizeof(T) + lane * 16) = res;
-      } else if (slot >= 0) {
-        const bool v = h >= a.hq + a.hk;
-        const int kh = h - a.hq - (v ? a.hk : 0);
-        *reinterpret_cast<uint4*>(a.pool + slot * a.pitch + (v ? a.plane : 0) +
-                                  (int64_t)kh * a.dim * sizeof(T) + lane * 16) = res;
-      }
+    for (int e = 0; e < N; e += 4) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(at + e));
+      f[e] = v.x;
+      f[e + 1] = v.y;
+      f[e + 2] = v.z;
+      f[e + 3] = v.w;
     }
   }
 }
 
-template <typename T, typename SI, typename PI>
-int launch_store(const QkStoreArgs& a, cudaStream_t s) {
-  int G = 1;
-  while (G * Vec16<T>::N < a.dim) G <<= 1;
-  const int heads = a.hq + 2 * a.hk, per_cta = kStoreThreads / G;
-  constexpr int H = 4;
-  const int64_t groups = a.tokens * ((heads + H - 1) / H);
-  int64_t grid = (groups + per_cta - 1) / per_cta;
-  const int64_t most = (int64_t)sm_count() * 8;
-  if (grid > most) grid = most;
-  return launch_rc(launch_pdl(qk_store_kernel<T, SI, PI, H>, dim3((unsigned)grid), dim3(kStoreThreads), 0, s, a, G),
-                   "qk_norm_rope_store");
+__device__ __forceinline__ int64_t index_at(const void* p, int bytes, uint32_t i) {
+  return bytes == 8 ? __ldg(static_cast<const long long*>(p) + i) : (int64_t)__ldg(static_cast<const int*>(p) + i);
 }
 
-template <typename T>
-int launch_store_idx(const QkStoreArgs& a, int slot_bytes, int position_bytes, cudaStream_t s) {
-  if (slot_bytes == 8)
-    return position_bytes == 8 ? launch_store<T, int64_t, int64_t>(a, s) : launch_store<T, int64_t, int32_t>(a, s);
-  return position_bytes == 8 ? launch_store<T, int32_t, int64_t>(a, s) : launch_store<T, int32_t, int32_t>(a, s);
+// G and the kind of pairs are compile-time: the shuffles of a loop whose length is
+// not cost more than the arithmetic (290 instructions a vector instead of about 100).
+template <typename T, int G, bool INTERLEAVED>
+__global__ void __launch_bounds__(kStoreThreads) qk_store_kernel(const QkStoreArgs a) {
+  using V = Vec16<T>;
+  constexpr int N = V::N, H = kStoreHeads;
+  grid_dep_wait();
+  grid_dep_launch();
+  const uint32_t g = blockIdx.x * (uint32_t)(kStoreThreads / G) + threadIdx.x / G;
+  const uint32_t t = a.part_div.div(g);
+  const int part = (int)(g - t * a.part_div.d);
+  const int qp = (a.hq + H - 1) / H, kp = (a.hk + H - 1) / H;
+  const int kind = part < qp ? 0 : (part < qp + kp ? 1 : 2);     // query, key, value
+  const int h0 = (kind == 0 ? part : kind == 1 ? part - qp : part - qp - kp) * H;
+  const int nh = t < a.tokens ? (kind ? a.hk : a.hq) - h0 : 0;   // heads from h0 on
+  const int lane = threadIdx.x % G, vecs = a.dim / N, half = a.rot / 2;
+  const bool live = lane < vecs;
+  const int row_head = (kind == 0 ? 0 : kind == 1 ? a.hq : a.hq + a.hk) + h0;
+  const char* row = a.qkv + (int64_t)t * a.qkv_pitch + (int64_t)row_head * (a.dim * (int)sizeof(T)) + lane * 16;
+  uint4 raw[H];
+#pragma unroll
+  for (int j = 0; j < H; ++j)
+    raw[j] = live && j < nh ? __ldg(reinterpret_cast<const uint4*>(row + j * a.dim * (int)sizeof(T))) : vzero();
+  int64_t slot = -1;
+  if (kind && nh > 0) {
+    slot = index_at(a.slots, a.slot_bytes, t);
+    if (slot >= a.pool_rows) {
+      if (lane == 0) atomicOr(&g_kvpool_status, 1u);
+      slot = -1;
+    }
+  }
+  // this lane's vector turns with its partner's: itself for pairs of neighbours
+  const int hv = half / N;
+  const bool turns = lane * N < a.rot;
+  const int partner = INTERLEAVED || !turns ? lane : (lane < hv ? lane + hv : lane - hv);
+  const void* w = kind ? a.k_weight : a.q_weight;
+  float c[N], s[N];                                              // times x and times its partner
+  bool rotates = false;
+  if (kind < 2) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      c[e] = 1.f;
+      s[e] = 0.f;
+    }
+    if (nh > 0) {
+      const int64_t pos = index_at(a.positions, a.position_bytes, t);
+      if (pos < 0 || pos >= a.max_pos) {
+        if (lane == 0 && a.rot > 0) atomicOr(&g_kvpool_status, 4u);
+      } else if (turns) {
+        rotates = true;
+        const float *cr = a.cos + pos * half, *sr = a.sin + pos * half;
+        if (INTERLEAVED) {
+          float cc[N / 2], ss[N / 2];
+          load_angles<N / 2>(cr + lane * (N / 2), cc);
+          load_angles<N / 2>(sr + lane * (N / 2), ss);
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            c[e] = cc[e / 2];
+            s[e] = e & 1 ? ss[e / 2] : -ss[e / 2];
+          }
+        } else {
+          const int at = (lane < hv ? lane : lane - hv) * N;
+          load_angles<N>(cr + at, c);
+          load_angles<N>(sr + at, s);
+          if (lane < hv) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) s[e] = -s[e];
+          }
+        }
+      }
+    }
+    if (w != nullptr && live) {
+      float wf[N], wp[N];
+      V::unpack(__ldg(reinterpret_cast<const uint4*>(w) + lane), wf);
+      V::unpack(__ldg(reinterpret_cast<const uint4*>(w) + partner), wp);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        c[e] *= wf[e];
+        s[e] *= wp[INTERLEAVED ? e ^ 1 : e];
+      }
+    }
+  }
+  const int head = a.dim * (int)sizeof(T);
+  char* dst = (kind == 0 ? a.q_out + ((int64_t)t * a.hq + h0) * head
+                         : a.pool + slot * a.pitch + (kind == 2 ? a.plane : 0) + (int64_t)h0 * head) +
+              lane * 16;
+  const bool stores = live && (kind == 0 || slot >= 0);
+  const bool norms = a.q_weight != nullptr || a.k_weight != nullptr;  // the same for every lane: shuffles stay whole
+  const bool some = __any_sync(0xffffffffu, kind < 2);          // a warp of values alone has nothing to work out
+#pragma unroll
+  for (int j = 0; j < H; ++j) {
+    float x[N], y[N], r = 1.f, down = 1.f;
+    uint4 other = raw[j];
+    if (!INTERLEAVED && some)
+      other = make_uint4(__shfl_sync(0xffffffffu, other.x, partner, G), __shfl_sync(0xffffffffu, other.y, partner, G),
+                         __shfl_sync(0xffffffffu, other.z, partner, G), __shfl_sync(0xffffffffu, other.w, partner, G));
+    V::unpack(raw[j], x);
+    if (norms && some) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < N; ++e) ss += x[e] * x[e];
+#pragma unroll
+      for (int d = G >> 1; d; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+      if (__any_sync(0xffffffffu, ss == INFINITY)) {  // squares past 32 bits: the same with x 2^-64
+        float st = 0.f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) st += (x[e] * 0x1p-64f) * (x[e] * 0x1p-64f);
+#pragma unroll
+        for (int d = G >> 1; d; d >>= 1) st += __shfl_xor_sync(0xffffffffu, st, d);
+        if (ss == INFINITY) {
+          ss = st;
+          down = 0x1p-64f;
+        }
+      }
+      r = rsqrtf(ss * a.inv_dim + a.eps * down * down);  // 2 ulp
+    }
+    if (!live || j >= nh) continue;
+    uint4 res = raw[j];
+    if (kind < 2 && (w != nullptr || rotates)) {
+      if (w == nullptr) {
+        down = 1.f;
+      } else if (down != 1.f) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] *= down;
+      }
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[e] *= c[e];
+      if (rotates) {
+        V::unpack(other, y);
+        if (down != 1.f) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) y[e] *= down;
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] += y[INTERLEAVED ? e ^ 1 : e] * s[e];
+      }
+      if (w != nullptr) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] *= r;
+      }
+      res = V::pack(x);
+    }
+    if (stores) *reinterpret_cast<uint4*>(dst + j * head) = res;
+  }
+}
+
+template <typename T, int G>
+int launch_store(QkStoreArgs a, cudaStream_t s) {
+  if constexpr (G > 1)
+    if (G / 2 * Vec16<T>::N >= a.dim) return launch_store<T, G / 2>(a, s);
+  const int qp = (a.hq + kStoreHeads - 1) / kStoreHeads, kp = (a.hk + kStoreHeads - 1) / kStoreHeads;
+  a.part_div = FastDiv((uint32_t)(qp + 2 * kp));
+  a.inv_dim = 1.f / (float)a.dim;
+  const int64_t groups = a.tokens * (qp + 2 * kp), per_cta = kStoreThreads / G;
+  GSEC_REQUIRE(groups < (1ll << 31), "qk_norm_rope_store: %lld tokens of %d heads are too many for one call",
+               (long long)a.tokens, a.hq + 2 * a.hk);
+  const dim3 grid((unsigned)((groups + per_cta - 1) / per_cta)), block(kStoreThreads);
+  return launch_rc(a.interleaved ? launch_pdl(qk_store_kernel<T, G, true>, grid, block, 0, s, a)
+                                 : launch_pdl(qk_store_kernel<T, G, false>, grid, block, 0, s, a),
+                   "qk_norm_rope_store");
 }
 
 }  // namespace
@@ -333,15 +377,15 @@ int slots_plan(const SlotPlanArgs& a, cudaStream_t s) {
   return launch_rc(launch_pdl(slots_plan_kernel, dim3((unsigned)grid), dim3(kPlanThreads), smem, s, a), "slots_plan");
 }
 
-int qk_norm_rope_store(const QkStoreArgs& a, int dtype, int slot_bytes, int position_bytes, cudaStream_t s) {
+int qk_norm_rope_store(const QkStoreArgs& a, int dtype, cudaStream_t s) {
   if (a.tokens == 0) return GSEC_OK;
   switch (dtype) {
     case GSEC_BF16:
-      return launch_store_idx<__nv_bfloat16>(a, slot_bytes, position_bytes, s);
+      return launch_store<__nv_bfloat16, 32>(a, s);
     case GSEC_F16:
-      return launch_store_idx<__half>(a, slot_bytes, position_bytes, s);
+      return launch_store<__half, 32>(a, s);
     default:
-      return launch_store_idx<float>(a, slot_bytes, position_bytes, s);
+      return launch_store<float, 32>(a, s);
   }
 }
 

@@ -105,8 +105,9 @@ struct QkStoreArgs {
   char* q_out;              // [tokens, hq, dim]
   char* pool;               // slot records: pitch bytes, V at + plane
   int64_t pitch, plane, pool_rows;
-  const void* slots;
+  const void* slots;        // int32 or int64
   const void* positions;
+  int slot_bytes, position_bytes;
   const float* cos;         // [max_pos, rot / 2]
   const float* sin;
   int rot;
@@ -115,10 +116,12 @@ struct QkStoreArgs {
   const void* k_weight;
   float eps;
   int interleaved;
+  FastDiv part_div;         // groups of heads per token
+  float inv_dim;
 };
 
 int slots_plan(const SlotPlanArgs& a, cudaStream_t s);
-int qk_norm_rope_store(const QkStoreArgs& a, int dtype, int slot_bytes, int position_bytes, cudaStream_t s);
+int qk_norm_rope_store(const QkStoreArgs& a, int dtype, cudaStream_t s);
 // Status bits of this file's kernels, at their place in the layout byte.
 unsigned kvpool_device_status(bool clear);
 
