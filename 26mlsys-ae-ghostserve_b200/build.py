@@ -2,6 +2,9 @@
 
     python 26mlsys-ae-ghostserve_b200/build.py [--force] [-v]
 
+(and lib/gsec_torch.so, the calls of the KV-pool operators from torch tensors,
+with g++ against torch's headers.)
+
 Each ``csrc/*.cu`` compiles to an object under ``_build/`` (skipped when newer
 than its sources and headers), then everything links into ``lib/libgsec.so``.
 The CUDA runtime is linked statically so the library only needs the driver at
@@ -26,6 +29,31 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CFLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-fvisibility=hidden",
           "-I", INCLUDE, "--expt-relaxed-constexpr"]
+
+
+BIND = os.path.join(CSRC, "bind.cpp")
+BIND_LIB = os.path.join(LIBDIR, "gsec_torch.so")
+
+
+def _build_bind(verbose: bool) -> None:
+    """lib/gsec_torch.so: a Python module on top of libgsec.so (found beside it at run time)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    inc = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(os.path.dirname(NVCC), "..", "include"),
+           INCLUDE]
+    cmd = ["g++", "-O2", "-std=c++20", "-fPIC", "-shared", "-fvisibility=hidden", "-Wno-deprecated",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{d}" for d in inc], BIND, "-o", BIND_LIB,
+           f"-L{torch_lib}", f"-L{LIBDIR}", "-l:libgsec.so", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+           "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {BIND}:\n{r.stdout}\n{r.stderr}")
 
 
 def _headers():
@@ -78,6 +106,8 @@ def build(force: bool = False, verbose: bool = False, ptxas_v: bool = False) -> 
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    if force or _stale(BIND_LIB, [BIND, *hdrs]):
+        _build_bind(verbose)
     return LIB
 
 

@@ -483,9 +483,14 @@ def test_refusals():
            dict(q=torch.zeros(3, 3, 64, device="cuda", dtype=BF)),
            dict(q=torch.zeros(3, 4, 68, device="cuda", dtype=BF)[:, :, 2:66]),
            dict(q=torch.zeros(3, 4, 12, device="cuda", dtype=BF), pool=torch.zeros(64, 2, 2, 12, device="cuda", dtype=BF))]
+    bad.append(dict(q=c["q"].clone().requires_grad_()))  # forward only
     for b in bad:
         with pytest.raises(ValueError):
             k.prefix_attention(**dict(c, **b))
+    with torch.no_grad():
+        k.prefix_attention(**dict(c, q=c["q"].clone().requires_grad_()))
+    with pytest.raises(ValueError):
+        k.prefix_attention(**c, scale=math.nan)
     qkv, pool, slots, positions, cos, sin, w = store_case(9, 4, 2, 64, 64, BF, True)
     base = dict(qkv=qkv, pool=pool, slots=slots, positions=positions, cos=cos, sin=sin, heads=4)
     for b in [dict(qkv=qkv.float()), dict(heads=5), dict(slots=slots[:8]), dict(slots=slots.short()),
