@@ -703,6 +703,11 @@ int gsec_prefix_attention(const void* q, int64_t q_pitch, int64_t q_head, int64_
   GSEC_REQUIRE(aligned16(q) && (q_pitch & 15) == 0 && (q_head & 15) == 0 && aligned16(out),
                "q, its strides and out must be 16-byte aligned");
   GSEC_REQUIRE(scale == scale && scale < 3e38f && scale > -3e38f, "scale must be finite");
+  const int64_t vec = (int64_t)dim * (dtype == GSEC_F32 ? 4 : 2);
+  if (hq == 1) q_head = vec;  // a stride that is never taken
+  if (tokens == 1) q_pitch = hq * q_head;
+  GSEC_REQUIRE(q_head >= vec && q_pitch >= vec && q_head < (1ll << 40) && q_pitch < (1ll << 40),
+               "q's strides must be at least a head's bytes and below 2^40");
   AttnArgs a{};
   a.q = static_cast<const char*>(q);
   a.q_pitch = q_pitch;

@@ -185,9 +185,12 @@ int attend_rows(const AttnArgs& a, cudaStream_t s) {
 // every role and 128-column bodies a one-tile segment took 12000 cycles).
 constexpr int kTileThreads = 384;   // 2 softmax warpgroups; a warp each issues products, loads K, loads V, walks and loads Q
 constexpr int kRows = 128, kKeys = 128, kBlock = 256;
-// Units of the line: a tile of a whole block; half a block's tile is three
-// quarters of that; a segment's beginning and end.
-constexpr int kUnitTile = 32, kUnitSegment = 16;
+// Units of the line: a tile of a whole block, half a block's tile being half of
+// that; a segment's beginning and end. (Three quarters and 16: 128 ragged decode
+// requests behind 2047 keys took 205 us instead of 145, 16 behind 32768 60 instead
+// of 50: the blocks of the prefix were late. With segments of 64 and more it is the
+// requests' own keys that are.)
+constexpr int kUnitTile = 32, kUnitSegment = 32;
 // Registers: a softmax thread holds 64 scores and 64 words of P. The launch has 168
 // per thread; the third warpgroup hands over what it does not need.
 constexpr int kLaunchRegs = 168, kSoftmaxRegs = 200, kOtherRegs = 104;
@@ -208,9 +211,14 @@ struct Start {           // a point on the line
   int y;                 // units into the segment
 };
 
+// Rows of a box of queries: a few, since a piece of a single token has `group` of them.
+constexpr int kQueryBox = 16;
+
 struct TilePlan {
   int run;               // rows of a box: the largest power of two dividing the page, at most a tile; 0: rows one by one
   int run_log;
+  int q_run;             // rows of a box of queries
+  int q_ratio;           // a token's pitch in head pitches: queries are loaded four rows at a time; 0: in boxes
   int slope;             // units by which a request's blocks grow
   int joint;             // prefix and own keys of a request are one segment (no stacking over requests)
   int ctas;
@@ -232,9 +240,11 @@ struct CutEnd {
 };
 
 // Tensor maps of the pool's K and V rows ([pool_rows, hk * dim], 128-byte
-// swizzle): boxes of 64 values x `run` rows, and single rows.
+// swizzle): boxes of 64 values x `run` rows, and single rows. The queries':
+// [tokens, hq, dim] in boxes of 64 values x `q_run` rows, or single rows.
 struct PoolMaps {
   CUtensorMap box[2], row[2];
+  CUtensorMap q;
 };
 
 __device__ __forceinline__ int tile_count(int keys) { return (keys + kKeys - 1) / kKeys; }
@@ -307,7 +317,7 @@ struct Walk {
   __device__ __forceinline__ int slope() const { return g.req < 0 ? 0 : p.slope; }
   __device__ __forceinline__ int units() const {
     const int u = base_units() + slope() * (g.blk + 1);
-    return kUnitSegment + (pair() ? u : u - u / 4);
+    return kUnitSegment + (pair() ? u : u / 2);
   }
   __device__ __forceinline__ int units_before(int m) const {
     return (int)((int64_t)m * (kUnitSegment + base_units()) + (int64_t)m * (m + 1) / 2 * slope());
@@ -411,6 +421,7 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, thread_wait(bar, parity, quit)) != 0;
 }
 
+constexpr int kBehind = 3 * 1024;  // bytes of shared memory behind the tiles (TileShared)
 template <int DP>
 struct TileShape {
   static constexpr int tile = kRows * DP * 2;                     // bytes of a Q, K or V tile
@@ -419,7 +430,7 @@ struct TileShape {
   static constexpr uint32_t ks = DP == 128 ? 2 : 6, vs = DP == 128 ? 3 : 6;
   static constexpr int stages = ks + vs;
   static constexpr int data = (2 + stages) * tile;
-  static constexpr int smem = data + 3072;
+  static constexpr int smem = data + kBehind;
 };
 
 // Shared memory behind the tiles.
@@ -434,22 +445,7 @@ struct TileShared {
   uint32_t tmem;
   int quit;
 };
-static_assert(sizeof(TileShared) <= 3072, "shared memory behind the tiles");
-
-// Scores of keys that the row does not see, from `cols` on, become -inf.
-__device__ __forceinline__ void mask_tile(uint32_t ts, int cols) {
-#pragma unroll 1
-  for (int k = 0; k < 128; k += 32) {
-    if (!__any_sync(0xffffffffu, cols < k + 32)) continue;
-    uint32_t x[32];
-    tc::ld32(ts + k, x);
-    tc::wait_ld(x);
-#pragma unroll
-    for (int e = 0; e < 32; ++e) x[e] = k + e < cols ? x[e] : 0xff800000u;
-    tc::st32(ts + k, x);
-  }
-  tc::wait_st();
-}
+static_assert(sizeof(TileShared) <= kBehind, "shared memory behind the tiles");
 
 // 16 words of P from 32 scores, their sum and their maximum (with `top`). (Two
 // scores to an instruction, fma.f32x2 and add.f32x2, took longer: 1550 cycles a
@@ -469,42 +465,52 @@ __device__ __forceinline__ float exp32(const uint32_t* x, uint32_t* w, float c, 
   return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
-// A tile whose maximum moves the reference of some row of the warp (or gives it
-// one): maximum first, then O and l to the new reference, then P.
+// A tile in two passes: where keys of it are hidden from some row of the warp
+// (those from column `cols` on), or its maximum moves the reference of one.
+// Maximum first, then O and l to the new reference, then P. Columns from `end` on
+// are no keys of any row, and no product takes them.
 template <typename T, int DP>
-__device__ __noinline__ float2 move_and_softmax(uint32_t ts, uint32_t to, float c, bool on, bool has_o, float m, float l) {
+__device__ __noinline__ float2 careful_tile(uint32_t ts, uint32_t to, float c, int cols, int end, bool on, bool has_o,
+                                            float m, float l) {
   uint32_t x[32], w[16];
-  float top = m;
+  float top = m, seen = -INFINITY, mc = 0.f;
 #pragma unroll 1
-  for (int k = 0; k < 128; k += 32) {
-    tc::ld32(ts + k, x);
-    tc::wait_ld(x);
-#pragma unroll
-    for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(x[e]));
-  }
-  const bool move = on && ((top - m) * c > 8.f || (m == -INFINITY && top > -INFINITY));
-  const float f = !move ? 1.f : (m == -INFINITY ? 0.f : tc::ex2((m - top) * c));
-  if (move) m = top;
-  l *= f;
-  if (has_o) {
+  for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll 1
-    for (int k = 0; k < DP; k += 32) {
-      tc::ld32(to + k, x);
+    for (int k = 0; k < end; k += 32) {
+      tc::ld32(ts + k, x);
       tc::wait_ld(x);
+      const int left = cols - k;
+      if (__any_sync(0xffffffffu, left < 32)) {
 #pragma unroll
-      for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
-      tc::st32(to + k, x);
+        for (int e = 0; e < 32; ++e) x[e] = e < left ? x[e] : 0xff800000u;
+      }
+      if (pass == 0) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(x[e]));
+      } else {
+        // P's words overlay the scores from the left, behind the reading
+        l += exp32<T>(x, w, c, mc, seen);
+        tc::st16(ts + k / 2, w);
+      }
     }
-  }
-  const float mc = m == -INFINITY ? 0.f : m * c;
-  float seen = -INFINITY;
-  // P's words overlay the scores from the left, behind the reading
+    if (pass == 0) {
+      const bool move = on && ((top - m) * c > 8.f || (m == -INFINITY && top > -INFINITY));
+      if (__any_sync(0xffffffffu, move)) {
+        const float f = !move ? 1.f : (m == -INFINITY ? 0.f : tc::ex2((m - top) * c));
+        if (move) m = top;
+        l *= f;
 #pragma unroll 1
-  for (int k = 0; k < 128; k += 32) {
-    tc::ld32(ts + k, x);
-    tc::wait_ld(x);
-    l += exp32<T>(x, w, c, mc, seen);
-    tc::st16(ts + k / 2, w);
+        for (int k = 0; has_o && k < DP; k += 32) {
+          tc::ld32(to + k, x);
+          tc::wait_ld(x);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+          tc::st32(to + k, x);
+        }
+      }
+      mc = m == -INFINITY ? 0.f : m * c;
+    }
   }
   tc::wait_st();
   return make_float2(m, l);
@@ -514,23 +520,31 @@ __device__ __noinline__ float2 move_and_softmax(uint32_t ts, uint32_t to, float 
 // 16-bit P there, (m, l) follow, and O at `to` (when it holds something) where the
 // reference moves. What a lane without a row (!on) computes is not read.
 //
-// P is taken relative to the reference m that the row has, while the tile's
-// maximum is found on the way: one pass over the scores, and no branch in it, so
-// that the exponentials of one part run under the loads, sums and conversions of
-// another (1300 cycles; 1900 in a loop over 64 columns; 1024 are the exponentials).
-// Only where the maximum turns out 8 binary places ahead, or the row has no
-// reference yet, is the reference moved and the tile done again; until then P
+// P is taken relative to the reference m that the row has, or to the largest of
+// its first 32 scores, while the tile's maximum is found on the way: one pass over
+// the scores, and no branch in it, so that the exponentials of one part run under
+// the loads, sums and conversions of another (1300 cycles; 1900 in a loop over 64
+// columns; 1024 are the exponentials). Only where the maximum turns out 8 binary
+// places ahead is the reference moved and the tile done again; until then P
 // exceeds 1, by 2^8 at most, which sums and 16-bit P hold as well as they hold 1.
 template <typename T, int DP>
-__device__ __forceinline__ void softmax_tile(uint32_t ts, uint32_t to, float c, bool on, bool has_o, float& m, float& l) {
-  bool again = __any_sync(0xffffffffu, on && m == -INFINITY);
+__device__ __forceinline__ void softmax_tile(uint32_t ts, uint32_t to, float c, int cols, int end, bool on, bool has_o,
+                                             float& m, float& l) {
+  bool again = __any_sync(0xffffffffu, cols < kKeys);
   if (!again) {
     uint32_t x[32], y[32], w[64];
-    const float mc = m == -INFINITY ? 0.f : m * c;
-    float top = m, sum;
     tc::ld32(ts, x);
     tc::wait_ld(x);
     tc::ld32(ts + 32, y);
+    if (__any_sync(0xffffffffu, m == -INFINITY)) {
+      float first = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 32; ++e) first = fmaxf(first, __uint_as_float(x[e]));
+      if (m == -INFINITY) m = first;
+      again = __any_sync(0xffffffffu, on && m == -INFINITY);
+    }
+    const float mc = m == -INFINITY ? 0.f : m * c;
+    float top = m, sum;
     sum = exp32<T>(x, w, c, mc, top);
     tc::wait_ld(y);
     tc::ld32(ts + 64, x);
@@ -540,7 +554,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t ts, uint32_t to, float c, 
     sum += exp32<T>(x, w + 32, c, mc, top);
     tc::wait_ld(y);
     sum += exp32<T>(y, w + 48, c, mc, top);
-    again = __any_sync(0xffffffffu, on && (top - m) * c > 8.f);
+    again = again || __any_sync(0xffffffffu, on && (top - m) * c > 8.f);
     if (!again) {
       l += sum;
       tc::st32(ts, w);
@@ -549,7 +563,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t ts, uint32_t to, float c, 
     }
   }
   if (again) {
-    const float2 r = move_and_softmax<T, DP>(ts, to, c, on, has_o, m, l);
+    const float2 r = careful_tile<T, DP>(ts, to, c, cols, end, on, has_o, m, l);
     m = r.x;
     l = r.y;
   }
@@ -594,6 +608,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
     tc::prefetch_map(maps.box + lane);
     tc::prefetch_map(maps.row + lane);
   }
+  if (warp == 11 && lane == 0) tc::prefetch_map(&maps.q);
   grid_dep_wait();
   grid_dep_launch();
 
@@ -704,14 +719,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
 #pragma unroll 1
         for (int i = two ? 0 : half; i < n; i += two ? 1 : 2) {
           const int cols = on ? piece_keys(g, i, a.prefix_len, see) : kKeys;
-          const bool cut = __any_sync(0xffffffffu, cols < kKeys);
+          const int keys = piece_keys(g, i, a.prefix_len, g.own), end = keys > 0 ? keys : 1;
           if (!(ok = warp_wait(sh.s_full + t, n_s & 1, quit))) break;
           ++n_s;
           tc::fence_after();
-          if (warp_on) {
-            if (cut) mask_tile(ts, cols);
-            softmax_tile<T, DP>(ts, to, c, on, two ? i > 0 : i >= 2, m, l);
-          }
+          if (warp_on) softmax_tile<T, DP>(ts, to, c, cols, end, on, two ? i > 0 : i >= 2, m, l);
           tc::fence_before();
           __syncwarp();
           if (lane == 0) pipe::bar_arrive(sh.p_full + t);
@@ -979,10 +991,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
           (void)pipe::bar_wait(sh.full + stage0 + q % turns, (q / turns) & 1);
     } else {
       // ------------------------------------------ the walk, loads of Q ----
-      constexpr int CH = DP / 8, RI = 32 / CH;                  // 16-byte chunks of a row; rows per instruction
-      const int ch = lane % CH, sub = lane / CH;
-      const bool in_dim = ch * 8 < a.dim;
-      const uint32_t panel = (uint32_t)(ch >> 3) * (kRows * 128);
+      // Row x of a block is head x % group of token x / group: boxes of whole groups
+      // over a few tokens (or of a part of a group) where that makes a power of two
+      // of rows, else four rows at a time.
+      constexpr int PN = DP / 64;
+      constexpr uint32_t kPanel = kRows * 128;
       Walk w(a, p, live);
       w.g = sh.first.g;
       int y = sh.first.y, left = x1 - x0, at = x0 - y;          // units into the segment, left of the stretch; its start
@@ -1029,32 +1042,44 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
         if (lane == 0) pipe::bar_arrive(sh.piece_full + slot);
         if (left <= 0) break;
         ++pi;
-        const int nq = nrow > kRows ? 2 : 1;
-        for (int b = 0; b < nq; ++b, ++n_q) {                   // only the rows that exist: a product's rows do not mix
-          const int buf = n_q & 1;
+        const int nq = nrow > kRows ? 2 : 1, head0 = w.g.kh * a.group;
+        for (int b = 0; b < nq; ++b, ++n_q) {                   // whole boxes of the rows that exist: a product's rows do not mix
+          const int buf = n_q & 1, here = nrow - b * kRows < kRows ? nrow - b * kRows : kRows;
+          const int xb = w.g.blk * kBlock + b * kRows;
+          uint32_t dst = base + buf * Shape::tile;
           if (n_q >= 2 && !(ok = warp_wait(sh.q_empty + buf, ((n_q >> 1) - 1) & 1, quit))) break;
-          const uint32_t dst = base + buf * Shape::tile + panel;
-          const int here = nrow - b * kRows < kRows ? nrow - b * kRows : kRows;
-          // row x is head x % group of token x / group; the next one of this lane's is RI further on
-          const int xs = w.g.blk * kBlock + b * kRows + sub, jt = (int)a.group_div.div((uint32_t)xs);
-          int hh = xs - jt * a.group;
-          const char* src = a.q + (int64_t)(w.g.tok + jt) * a.q_pitch + (int64_t)(w.g.kh * a.group + hh) * a.q_head + ch * 16;
-          const int64_t wrap = a.q_pitch - (int64_t)a.group * a.q_head, on_by = RI * a.q_head;
-#pragma unroll 4
-          for (int rr = sub; rr < here; rr += RI) {
-            if (in_dim) tc::copy16(dst + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4), src, true);
-            src += on_by;
-            hh += RI;
-            while (hh >= a.group) {
-              hh -= a.group;
-              src += wrap;
+          if (p.q_ratio > 0) {
+            int4 z;
+            int* zj = &z.x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int x = xb + lane * 4 + j, jt = (int)a.group_div.div((uint32_t)x);
+              zj[j] = (w.g.tok + jt) * p.q_ratio + head0 + x - jt * a.group;
+            }
+            if (tc::elect()) pipe::bar_expect_tx(sh.q_full + buf, (uint32_t)((here + 3) / 4 * 512 * PN));
+            __syncwarp();
+#pragma unroll 1
+            for (int q = 0; q < (here + 3) / 4; ++q, dst += 512) {
+              const int4 y4 = make_int4(__shfl_sync(0xffffffffu, z.x, q), __shfl_sync(0xffffffffu, z.y, q),
+                                        __shfl_sync(0xffffffffu, z.z, q), __shfl_sync(0xffffffffu, z.w, q));
+              if (tc::elect()) {
+#pragma unroll
+                for (int pn = 0; pn < PN; ++pn) tc::load_rows(dst + pn * kPanel, &maps.q, pn * 64, y4, sh.q_full + buf);
+              }
+              __syncwarp();
+            }
+          } else if (tc::elect()) {
+            const int boxes = (here + p.q_run - 1) / p.q_run;
+            pipe::bar_expect_tx(sh.q_full + buf, (uint32_t)(boxes * p.q_run * 128 * PN));
+#pragma unroll 1
+            for (int q = 0; q < boxes; ++q, dst += p.q_run * 128) {
+              const int x = xb + q * p.q_run, jt = (int)a.group_div.div((uint32_t)x);
+#pragma unroll
+              for (int pn = 0; pn < PN; ++pn)
+                tc::load_box3(dst + pn * kPanel, &maps.q, pn * 64, head0 + x - jt * a.group, w.g.tok + jt, sh.q_full + buf);
             }
           }
-          tc::copy_commit();
-          tc::copy_wait<0>();
-          tc::fence_async();
           __syncwarp();
-          if (lane == 0) pipe::bar_arrive(sh.q_full + buf);
         }
         if (!ok) break;
         left -= units - y;
@@ -1062,6 +1087,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
         y = 0;
         if (left > 0) w.next();
       }
+      if (*quit)
+        for (uint32_t q = n_q > 2 ? n_q - 2 : 0; q < n_q; ++q) (void)pipe::bar_wait(sh.q_full + (q & 1), (q >> 1) & 1);
     }
     }
   }
@@ -1262,21 +1289,37 @@ EncodeTiled encode_tiled() {
   return fn;
 }
 
-bool pool_map(CUtensorMap* m, bool bf16, const char* at, int64_t values, int64_t rows, int64_t pitch, int box_rows) {
-  const cuuint64_t size[2] = {(cuuint64_t)values, (cuuint64_t)rows}, stride[1] = {(cuuint64_t)pitch};
-  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, step[2] = {1, 1};
+// Map of N dimensions of 16-bit values at `at`, 64 values wide in a box.
+template <int N>
+bool tile_map(CUtensorMap* m, bool bf16, const char* at, const cuuint64_t (&size)[N], const cuuint64_t (&stride)[N - 1],
+              const cuuint32_t (&box)[N]) {
+  cuuint32_t step[N];
+  for (int i = 0; i < N; ++i) step[i] = 1;
   const EncodeTiled encode = encode_tiled();
   return encode != nullptr &&
-         encode(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-                const_cast<char*>(at), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+         encode(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, N, const_cast<char*>(at),
+                size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool query_map(CUtensorMap* m, bool bf16, const AttnArgs& a, const TilePlan& p) {
+  using Z = cuuint64_t;
+  if (p.q_ratio > 0)
+    return tile_map<2>(m, bf16, a.q, {(Z)a.dim, (Z)((a.tokens - 1) * p.q_ratio + a.hq)}, {(Z)a.q_head}, {64, 1});
+  const int heads = a.group < p.q_run ? a.group : p.q_run;
+  return tile_map<3>(m, bf16, a.q, {(Z)a.dim, (Z)a.hq, (Z)a.tokens}, {(Z)a.q_head, (Z)a.q_pitch},
+                     {64, (cuuint32_t)heads, (cuuint32_t)(p.q_run / heads)});
 }
 
 template <typename T, int DP>
 int launch_tiles(const AttnArgs& a, cudaStream_t s) {
   int64_t bytes = 0;
-  const TilePlan p = tile_plan(a, &bytes);
+  TilePlan p = tile_plan(a, &bytes);
+  const int even = a.group & -a.group;  // heads of a box: a power of two
+  p.q_run = even < kQueryBox && even < a.group ? even : kQueryBox;
+  p.q_ratio = p.q_run < 4 && a.q_pitch % a.q_head == 0 && a.tokens * (a.q_pitch / a.q_head) < INT_MAX
+                  ? (int)(a.q_pitch / a.q_head)
+                  : 0;
   // the line is counted in 32 bits
   const int64_t keys = (int64_t)a.prefix_len + (int64_t)a.width * a.page;
   const int64_t blocks = a.tokens * a.group / kBlock + a.batch + 1;  // of the requests, and of the prefix
@@ -1288,12 +1331,12 @@ int launch_tiles(const AttnArgs& a, cudaStream_t s) {
   bool ok = true;
   for (int kv = 0; kv < 2; ++kv) {
     const char* at = a.pool + (kv ? a.plane : 0);
-    const int64_t values = (int64_t)a.hk * a.dim;
-    ok = ok && pool_map(maps.box + kv, Vec16<T>::bf16, at, values, a.pool_rows, a.pitch, p.run ? p.run : 1) &&
-         pool_map(maps.row + kv, Vec16<T>::bf16, at, values, a.pool_rows, a.pitch, 1);
+    const cuuint64_t size[2] = {(cuuint64_t)a.hk * a.dim, (cuuint64_t)a.pool_rows}, pitch[1] = {(cuuint64_t)a.pitch};
+    ok = ok && tile_map<2>(maps.box + kv, Vec16<T>::bf16, at, size, pitch, {64, (cuuint32_t)(p.run ? p.run : 1)}) &&
+         tile_map<2>(maps.row + kv, Vec16<T>::bf16, at, size, pitch, {64, 1});
   }
-  if (!ok) {
-    set_error("prefix_attention: the pool's tensor maps were refused");
+  if (!ok || !query_map(&maps.q, Vec16<T>::bf16, a, p)) {
+    set_error("prefix_attention: the tensor maps of pool and queries were refused");
     return GSEC_ECUDA;
   }
   constexpr int smem = TileShape<DP>::smem;

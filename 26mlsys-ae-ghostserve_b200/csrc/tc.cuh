@@ -138,6 +138,14 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
       ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(smem_addr(bar))
       : "memory");
 }
+// The same of three dimensions.
+__device__ __forceinline__ void load_box3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+      : "memory");
+}
+
 // Four rows of a tensor map (box one row high), one after the other; a row outside the map is zeros.
 __device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, int x, const int4& y, uint64_t* bar) {
   asm volatile(

@@ -21,7 +21,7 @@ def plan_args(**kw):
 
 
 def store_args(**kw):
-    d = dict(qkv=A[0], pitch=3072, tokens=4, dtype=0, hq=8, hk=2, dim=128, q_out=A[1], pool=A[2], slot_pitch=1024,
+    d = dict(qkv=A[0], pitch=12 * 128 * 2, tokens=4, dtype=0, hq=8, hk=2, dim=128, q_out=A[1], pool=A[2], slot_pitch=1024,
              plane=512, rows=100, slots=A[3], slot_bytes=8, positions=A[4], position_bytes=4, cos=A[5], sin=A[6],
              rot=128, max_pos=64, qw=None, kw=None, eps=1e-5, interleaved=0, stream=None)
     d.update(kw)
