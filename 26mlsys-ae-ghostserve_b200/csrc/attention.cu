@@ -16,18 +16,14 @@ static __device__ unsigned g_attn_status;
 
 namespace {
 
-// Slot of key x of request r (prefix first), or -1 (flagged) for a page outside the pool.
+// Slot of key x of request r (prefix first), or -1 for a page outside the pool.
 __device__ __forceinline__ int64_t key_slot(const AttnArgs& a, int r, int32_t x) {
   const int32_t own = x - a.prefix_len;
   const uint32_t y = own < 0 ? (uint32_t)x : (uint32_t)own;
   const uint32_t pi = a.page_div.div(y);
   const int32_t page = own < 0 ? __ldg(a.prefix + pi) : __ldg(a.table + r * a.table_pitch + pi);
   const int64_t slot = (int64_t)page * a.page + (y - pi * a.page);
-  if (page < 0 || slot >= a.pool_rows) {
-    atomicOr(&g_attn_status, 1u);
-    return -1;
-  }
-  return slot;
+  return page < 0 || slot >= a.pool_rows ? -1 : slot;
 }
 
 // ------------------------------------------------------ one row per CTA -------
@@ -85,6 +81,7 @@ __global__ void __launch_bounds__(kRowThreads) attend_row_kernel(const AttnArgs 
   for (int it = 0; it < rounds; ++it) {
     const int32_t x = it * ngrp + grp;
     const int64_t slot = x < keys ? key_slot(a, r, x) : -1;
+    if (x < keys && slot < 0) atomicOr(&g_attn_status, 1u);
     const char* rec = a.pool + slot * a.pitch + (int64_t)kh * a.dim * sizeof(T);
     float k[E], v[E], s = 0.f;
 #pragma unroll
@@ -383,6 +380,7 @@ struct alignas(16) Piece {
   int req, more, len;    // row x sees own keys below more + x / group + 1 (at most len)
   int kind;              // 1: the rows' only segment, in one piece; 2: its last piece; 4: the segment in one piece
   int c0;                // first CTA of the segment
+  int tail[2], tail_keys[2];  // the last tile of the prefix and of the own keys, and their sixteens
 };
 constexpr int kPieces = 4;
 
@@ -399,26 +397,34 @@ __device__ __forceinline__ int piece_keys(const Piece& g, int i, int prefix_len,
 // Keys of a tile as the products take them: sixteens, at least one.
 __device__ __forceinline__ int sixteens(int keys) { return keys <= 16 ? 1 : (keys + 15) >> 4; }
 
+__device__ __forceinline__ int tile_sixteens(const Piece& g, int i) {
+  return i == g.tail[0] ? g.tail_keys[0] : (i == g.tail[1] ? g.tail_keys[1] : kKeys / 16);
+}
+
 __device__ __forceinline__ int share(int total, int ctas) {
   const int n = (total + ctas - 1) / ctas;
   return n < kMinShare ? kMinShare : n;
 }
 
-// A wait gives up after 2^24 turns (about a second) and raises `quit`, which ends
-// every other wait of the CTA.
-__device__ __forceinline__ bool thread_wait(uint64_t* bar, uint32_t parity, volatile int* quit) {
+// A wait gives up after 2^24 turns and raises `quit`, which ends every other wait
+// of the CTA.
+__device__ __forceinline__ bool long_wait(uint64_t* bar, uint32_t parity, volatile int* quit) {
 #pragma unroll 1
   for (int i = 0; i < 1 << 24; ++i) {
     if (pipe::bar_try(bar, parity)) return true;
     if (*quit) return false;
   }
   *quit = 1;
-  atomicOr(&g_attn_status, 2u);
   return false;
+}
+// Of the thread that issues the products, whose barriers are mostly through: a
+// wait on such a one costs some 200 cycles, a test 50.
+__device__ __forceinline__ bool thread_wait(uint64_t* bar, uint32_t parity, volatile int* quit) {
+  return pipe::bar_test(bar, parity) || long_wait(bar, parity, quit);
 }
 // Every lane of the warp gets the same answer.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* quit) {
-  return __all_sync(0xffffffffu, thread_wait(bar, parity, quit)) != 0;
+  return __all_sync(0xffffffffu, long_wait(bar, parity, quit)) != 0;
 }
 
 constexpr int kBehind = 3 * 1024;  // bytes of shared memory behind the tiles (TileShared)
@@ -443,7 +449,8 @@ struct TileShared {
   Start first;                      // where this CTA's stretch starts
   int total;
   uint32_t tmem;
-  int quit;
+  int quit;                         // a wait gave up
+  int bad;                          // a page was outside the pool
 };
 static_assert(sizeof(TileShared) <= kBehind, "shared memory behind the tiles");
 
@@ -569,7 +576,8 @@ __device__ __forceinline__ void softmax_tile(uint32_t ts, uint32_t to, float c, 
   }
 }
 
-template <typename T, int DP>
+// ROWS: pages of less than eight rows, loaded four rows at a time.
+template <typename T, int DP, bool ROWS>
 __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const AttnArgs a, const TilePlan p,
                                                                      const __grid_constant__ PoolMaps maps) {
   using Shape = TileShape<DP>;
@@ -598,7 +606,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
     pipe::bar_init(&sh.taken, 4);
     pipe::bar_init_fence();
     sh.quit = (tc::smem_addr(smem) & 1023u) != 0;  // the swizzle counts from 1024-byte patterns
-    if (sh.quit) atomicOr(&g_attn_status, 2u);
+    sh.bad = 0;
   }
   if (warp == 8) {
     tc::alloc(&sh.tmem, 512);
@@ -829,20 +837,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
       // -------------------------------------------------------- products ----
       // One thread. Step s runs on S, P and O number s & 1; its scores are issued
       // right after the P V of step s - 2. A lone thread takes five cycles and more
-      // for an instruction, so the loop is kept short.
+      // for an instruction, so what can be done before P arrives is, and the
+      // products are unrolled.
       if (tc::elect()) {
         const uint32_t id_s = tc::idesc(Vec16<T>::bf16, kRows, 0, false, a.scale < 0.f);
         const uint32_t id_o = tc::idesc(Vec16<T>::bf16, kRows, a.dim, true);
         const int ks = a.dim / 16;
         const uint64_t qdesc = tc::desc(base, 16, 1024), kdesc = tc::desc(ring, 16, 1024),
-                       vdesc = tc::desc(ring, kKeys * 128, 1024);
-        uint32_t n_o0 = 0, n_o1 = 0, n_q = 0;                   // uses of the O's, Q tiles
-        // the scores' place: piece, tiles so far, tile, step of the tile; the sums' place
-        uint32_t qp = 0, qat = 0, wp = 0, wat = 0;
-        int qi = 0, qsub = 0, qn = 0, wi = 0, wsub = 0, wn = 0;
-        bool qtwo = false, wtwo = false;
+                       vdesc = tc::desc(ring + KS * Shape::tile, kKeys * 128, 1024);
+        uint32_t n_o0 = 0, n_o1 = 0, n_q = 0, id = 0;                   // uses of the O's, Q tiles
+        // the scores' place: piece, tile of it, step of the tile; the sums' place
+        uint32_t qp = 0, wp = 0;
+        int qi = 0, qsub = 0, qn = 0, wi = 0, wsub = 0, wn = 0, kk = 0;
+        uint32_t k_st = 0, k_turn = 0, v_st = 0, v_turn = 0;    // ring stages and the parity of their turns
+        bool qtwo = false, wtwo = false, have = false;          // have: the scores' piece is known
         for (uint32_t s = 0;; ++s) {                            // sums of step s - 2, scores of step s
           const uint32_t l2 = s & 1;
+          bool ready = false;                                   // the scores' operands are there
+          const auto open_piece = [&] {
+            const Piece& g = sh.piece[qp % kPieces];
+            qn = g.n;
+            qtwo = g.nrow > kRows;
+            have = true;
+          };
           if (s >= 2) {
             if (wi == 0 && wsub == 0) {
               if (!thread_wait(sh.piece_full + wp % kPieces, (wp / kPieces) & 1, quit)) break;
@@ -850,64 +867,70 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
               if (wn == 0) break;
               wtwo = sh.piece[wp % kPieces].nrow > kRows;
             }
-            const Piece& g = sh.piece[wp % kPieces];
-            const uint32_t st = KS + wat % VS;
             const bool fresh = wi < (wtwo ? 1 : 2), last = wi >= wn - (wtwo ? 1 : 2), tile_done = !wtwo || wsub;
-            const int kk = sixteens(piece_keys(g, wi, a.prefix_len, g.own));
-            if (!thread_wait(sh.full + st, (wat / VS) & 1, quit)) break;
+            if (wsub == 0) {
+              kk = tile_sixteens(sh.piece[wp % kPieces], wi);
+              if (!thread_wait(sh.full + KS + v_st, v_turn, quit)) break;
+            }
             if (fresh) {
               const uint32_t uses = l2 ? n_o1 : n_o0;
               if (uses > 0 && !thread_wait(sh.o_empty + l2, (uses - 1) & 1, quit)) break;
               n_o0 += l2 ^ 1;
               n_o1 += l2;
             }
+            if (!have && pipe::bar_test(sh.piece_full + qp % kPieces, (qp / kPieces) & 1)) open_piece();
+            ready = have && qn > 0 && (qsub || pipe::bar_test(sh.full + k_st, k_turn)) &&
+                    (qi > 0 || pipe::bar_test(sh.q_full + ((n_q + qsub) & 1), ((n_q + qsub) >> 1) & 1));
+            const uint64_t vd = vdesc + v_st * (Shape::tile >> 4);
+            const uint32_t o = tmem + 256 + l2 * 128, pa = tmem + l2 * 128;
             if (!thread_wait(sh.p_full + l2, ((s - 2) >> 1) & 1, quit)) break;
             tc::fence_after();
-            uint64_t vd = vdesc + st * (Shape::tile >> 4);
-            const uint32_t o = tmem + 256 + l2 * 128, pa = tmem + l2 * 128;
-#pragma unroll 4
-            for (int j = 0; j < kk; ++j, vd += 2048 >> 4) tc::mma_ts(o, pa + j * 8, vd, id_o, !fresh || j > 0);
-            if (tile_done) tc::commit(sh.empty + st);
+            if (kk == kKeys / 16) {
+#pragma unroll
+              for (int j = 0; j < kKeys / 16; ++j) tc::mma_ts(o, pa + j * 8, vd + j * (2048 >> 4), id_o, !fresh || j > 0);
+            } else {
+#pragma unroll 1
+              for (int j = 0; j < kk; ++j) tc::mma_ts(o, pa + j * 8, vd + j * (2048 >> 4), id_o, !fresh || j > 0);
+            }
+            if (tile_done) tc::commit(sh.empty + KS + v_st);
             if (last) tc::commit(sh.o_full + l2);
             wsub = !tile_done;
             if (tile_done) {
-              ++wat;
+              if (++v_st == VS) {
+                v_st = 0;
+                v_turn ^= 1;
+              }
               if (++wi == wn) {
                 wi = 0;
                 pipe::bar_arrive(sh.piece_empty + wp++ % kPieces);
               }
             }
           }
-          if (qn < 0) continue;                                 // behind the last piece
-          if (qi == 0 && qsub == 0) {
-            if (!thread_wait(sh.piece_full + qp % kPieces, (qp / kPieces) & 1, quit)) break;
-            qn = sh.piece[qp % kPieces].n;
-            qtwo = sh.piece[qp % kPieces].nrow > kRows;
-            if (qn == 0) {
-              qn = -1;
-              continue;
+          if (!ready) {
+            if (!have) {
+              if (!thread_wait(sh.piece_full + qp % kPieces, (qp / kPieces) & 1, quit)) break;
+              open_piece();
             }
+            if (qn == 0) continue;                              // behind the last piece
+            if (qi == 0 && !thread_wait(sh.q_full + ((n_q + qsub) & 1), ((n_q + qsub) >> 1) & 1, quit)) break;
+            if (!thread_wait(sh.full + k_st, k_turn, quit)) break;
           }
-          const uint32_t nq = n_q + qsub, st = qat % KS;
-          if (qi == 0 && !thread_wait(sh.q_full + (nq & 1), (nq >> 1) & 1, quit)) break;
-          if (!thread_wait(sh.full + st, (qat / KS) & 1, quit)) break;
-          tc::fence_after();
-          const Piece& g = sh.piece[qp % kPieces];
-          const uint32_t id = id_s | (uint32_t)(2 * sixteens(piece_keys(g, qi, a.prefix_len, g.own))) << 17;
-          uint64_t qd = qdesc + (nq & 1) * (Shape::tile >> 4), kd = kdesc + st * (Shape::tile >> 4);
-#pragma unroll 4
-          for (int j = 0; j < ks; ++j) {
-            tc::mma_ss(tmem + l2 * 128, qd, kd, id, j > 0);
-            const uint32_t by = (j & 3) == 3 ? (kRows * 128 - 96) >> 4 : 2;  // 32 bytes on, or to the next 64 values
-            qd += by;
-            kd += by;
+          if (qsub == 0) id = id_s | (uint32_t)(2 * tile_sixteens(sh.piece[qp % kPieces], qi)) << 17;
+          const uint64_t qd = qdesc + ((n_q + qsub) & 1) * (Shape::tile >> 4), kd = kdesc + k_st * (Shape::tile >> 4);
+#pragma unroll
+          for (int j = 0; j < DP / 16; ++j) {                   // 32 bytes on, or to the next 64 values
+            const int at = (j & 3) * 2 + (j >> 2) * (kRows * 128 >> 4);
+            if (j < ks) tc::mma_ss(tmem + l2 * 128, qd + at, kd + at, id, j > 0);
           }
           const bool tile_done = !qtwo || qsub, done = tile_done && qi == qn - 1;
           tc::commit(sh.s_full + l2);
-          if (tile_done) tc::commit(sh.empty + st);
+          if (tile_done) tc::commit(sh.empty + k_st);
           qsub = !tile_done;
           if (tile_done) {
-            ++qat;
+            if (++k_st == KS) {
+              k_st = 0;
+              k_turn ^= 1;
+            }
             ++qi;
           }
           if (done) {
@@ -915,6 +938,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
             if (qtwo) tc::commit(sh.q_empty + ((n_q + 1) & 1));
             n_q += qtwo ? 2 : 1;
             qi = 0;
+            have = false;
             pipe::bar_arrive(sh.piece_empty + qp++ % kPieces);
           }
         }
@@ -942,24 +966,32 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
 #pragma unroll 1
         for (int i = 0; i < n; ++i, ++pos) {
           const int k0 = piece_key0(g, i) + (g.off + i < g.np ? 0 : a.prefix_len), valid = piece_keys(g, i, a.prefix_len, g.own);
-          int boxes = p.run > 0 ? valid / p.run : 0;
-          int32_t y = 0;
-          if (lane < boxes) {
-            const int64_t sl = key_slot(a, g.req, k0 + lane * p.run);
-            y = sl < 0 || sl + p.run > a.pool_rows ? -1 : (int32_t)sl;
+          int boxes = 0;
+          if (!ROWS) {
+            boxes = valid >> p.run_log;
+            int32_t y = 0;
+            if (lane < boxes) {
+              const int64_t sl = key_slot(a, g.req, k0 + (lane << p.run_log));
+              y = sl < 0 || sl + p.run > a.pool_rows ? -1 : (int32_t)sl;
+            }
+            if (__any_sync(0xffffffffu, y < 0)) boxes = 0;
+            if (lane < boxes) rows[lane] = y;
           }
-          if (__any_sync(0xffffffffu, y < 0)) boxes = 0;
-          if (lane < boxes) rows[lane] = y;
-          const int quad0 = boxes * p.run / 4, quads = sixteens(valid) * 4;
+          const int quad0 = (boxes << p.run_log) >> 2, quads = sixteens(valid) * 4;
           if (lane >= quad0 && lane < quads) {
             int32_t* z = rows + lane * 4;                       // behind the boxes' entries
+            const auto look = [&](int j) {
+              const bool is = lane * 4 + j < valid;
+              const int64_t sl = is ? key_slot(a, g.req, k0 + lane * 4 + j) : -1;
+              if (is && sl < 0) sh.bad = 1;
+              z[j] = sl < 0 ? none : (int32_t)sl;
+            };
+            if (ROWS) {                                         // four lookups in flight
+#pragma unroll
+              for (int j = 0; j < 4; ++j) look(j);
+            } else {
 #pragma unroll 1
-            for (int j = 0; j < 4; ++j) {
-              z[j] = none;
-              if (lane * 4 + j < valid) {
-                const int64_t sl = key_slot(a, g.req, k0 + lane * 4 + j);
-                if (sl >= 0) z[j] = (int32_t)sl;
-              }
+              for (int j = 0; j < 4; ++j) look(j);
             }
           }
           const uint32_t st = stage0 + pos % turns;
@@ -1021,8 +1053,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
           if (left > 0) {
             const bool whole = end - off == w.g.tiles;
             g.off = off;
-            g.np = w.prefix_part();
-            g.own = w.own_keys();
+            const int np = w.prefix_part(), own = w.own_keys();
+            g.np = np;
+            g.own = own;
+            g.tail[0] = np - 1 - off;
+            g.tail_keys[0] = sixteens(a.prefix_len - (np - 1) * kKeys);
+            g.tail[1] = w.g.tiles - 1 - off;
+            g.tail_keys[1] = sixteens(own - (w.g.tiles - 1 - np) * kKeys);
             g.x0 = w.g.blk * kBlock;
             g.nrow = nrow;
             g.tok = w.g.tok;
@@ -1104,6 +1141,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
   __syncthreads();
   tc::fence_after();
   if (warp == 8) tc::dealloc(tmem, 512);
+  if (tid == 0 && (sh.quit || sh.bad)) atomicOr(&g_attn_status, (sh.quit ? 2u : 0u) | (sh.bad ? 1u : 0u));
 }
 
 // ------------------------------------------------------------ joining parts ---
@@ -1340,21 +1378,25 @@ int launch_tiles(const AttnArgs& a, cudaStream_t s) {
     return GSEC_ECUDA;
   }
   constexpr int smem = TileShape<DP>::smem;
-  if (launch_cache().blocks_per_sm(attend_tile_kernel<T, DP>, kTileThreads, smem) < 0)
+  const auto kernel = p.run ? attend_tile_kernel<T, DP, false> : attend_tile_kernel<T, DP, true>;
+  if (launch_cache().blocks_per_sm(kernel, kTileThreads, smem) < 0)
     return check_launch("attend_tile launch shape");
   // a smaller launch would leave the softmax warpgroups waiting for registers that are not there
   static const bool regs_ok = [] {
-    cudaFuncAttributes at{};
-    return cudaFuncGetAttributes(&at, attend_tile_kernel<T, DP>) == cudaSuccess && at.numRegs == kLaunchRegs;
+    cudaFuncAttributes x{}, y{};
+    return cudaFuncGetAttributes(&x, attend_tile_kernel<T, DP, false>) == cudaSuccess && x.numRegs == kLaunchRegs &&
+           cudaFuncGetAttributes(&y, attend_tile_kernel<T, DP, true>) == cudaSuccess && y.numRegs == kLaunchRegs;
   }();
   GSEC_REQUIRE(regs_ok, "attend_tile: launch registers are not %d", kLaunchRegs);
   const int rc = launch_rc(
-      launch_pdl(attend_tile_kernel<T, DP>, dim3((unsigned)p.ctas), dim3(kTileThreads), smem, s, a, p, maps),
+      launch_pdl(kernel, dim3((unsigned)p.ctas), dim3(kTileThreads), smem, s, a, p, maps),
       "prefix_attention");
   if (rc) return rc;
-  if (p.joint)
-    return launch_rc(launch_pdl(attend_join_cuts_kernel<T>, dim3((unsigned)p.ctas, 8), dim3(256), 0, s, a, p),
+  if (p.joint) {  // a warp to a row of a whole block, or a block to a row of a few
+    const unsigned y = a.tokens * a.group < kBlock ? 8 : kBlock / 8;
+    return launch_rc(launch_pdl(attend_join_cuts_kernel<T>, dim3((unsigned)p.ctas, y), dim3(256), 0, s, a, p),
                      "prefix_attention join");
+  }
   const int64_t rows = a.tokens * a.hq;
   // few rows: eight warps to a row, since each may have a part from every CTA
   if (rows <= (int64_t)p.ctas * 16)
