@@ -885,13 +885,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
             const uint32_t o = tmem + 256 + l2 * 128, pa = tmem + l2 * 128;
             if (!thread_wait(sh.p_full + l2, ((s - 2) >> 1) & 1, quit)) break;
             tc::fence_after();
-            if (kk == kKeys / 16) {
-#pragma unroll
-              for (int j = 0; j < kKeys / 16; ++j) tc::mma_ts(o, pa + j * 8, vd + j * (2048 >> 4), id_o, !fresh || j > 0);
-            } else {
 #pragma unroll 1
-              for (int j = 0; j < kk; ++j) tc::mma_ts(o, pa + j * 8, vd + j * (2048 >> 4), id_o, !fresh || j > 0);
-            }
+            for (int j = 0; j < kk; ++j) tc::mma_ts(o, pa + j * 8, vd + j * (2048 >> 4), id_o, !fresh || j > 0);
             if (tile_done) tc::commit(sh.empty + KS + v_st);
             if (last) tc::commit(sh.o_full + l2);
             wsub = !tile_done;
