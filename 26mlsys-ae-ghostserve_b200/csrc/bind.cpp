@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
@@ -23,6 +24,7 @@
 namespace {
 
 PyObject* g_check = nullptr;  // _lib.check: raises for a return code
+PyTypeObject* g_plan = nullptr;  // kvpool.SlotPlan
 
 struct Refused {};  // a Python exception is set
 
@@ -90,9 +92,18 @@ struct Call {
   }
   void* stream() const { return c10::cuda::getCurrentCUDAStream(device.index()).stream(); }
   at::Tensor empty(at::IntArrayRef shape, at::ScalarType type) const {
-    return at::empty(shape, at::TensorOptions().dtype(type).device(device));
+    return at::detail::empty_cuda(shape, type, device, std::nullopt);
   }
 };
+
+// Elements [from, from + count) of a new one-dimensional tensor, as a tensor of
+// their own. (A split through the dispatcher took 2 us.)
+at::Tensor piece(const at::Tensor& t, int64_t from, int64_t count) {
+  at::Tensor r = at::detail::make_tensor<at::TensorImpl>(at::TensorImpl::VIEW, at::Storage(t.storage()), t.key_set(), t.dtype());
+  r.unsafeGetTensorImpl()->set_storage_offset(from);
+  r.unsafeGetTensorImpl()->set_sizes_contiguous({count});
+  return r;
+}
 
 void finish(int rc) {
   if (rc == GSEC_OK) return;
@@ -162,7 +173,7 @@ bool count_is(Py_ssize_t n, Py_ssize_t want) {
   return false;
 }
 
-// (lens, new, table, free, cursor, page, tokens, base) -> (slots, positions, cu, lens, cursor)
+// (lens, new, table, free, cursor, page, tokens, base) -> SlotPlan(slots, positions, cu, lens, cursor, table, page)
 PyObject* slots_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!count_is(n, 8)) return nullptr;
   return guarded([&]() -> PyObject* {
@@ -182,15 +193,25 @@ PyObject* slots_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
     at::Tensor slots = c.empty({tokens}, at::kLong);
     // the int32 outputs share one allocation, the per-token one in front
     at::Tensor rest = c.empty({tokens + 2 * batch + 2}, at::kInt);
-    std::vector<at::Tensor> o = rest.split_with_sizes({tokens, batch + 1, batch, 1});
+    const int64_t sizes[4] = {tokens, batch + 1, batch, 1};
     auto* at = static_cast<int32_t*>(rest.data_ptr());
     finish(gsec_slots_plan(lens_at, new_at, (int32_t)batch, t.at, t.pitch, t.width, free_at, pages.numel(), cursor_at,
                            page, base, static_cast<int64_t*>(slots.data_ptr()), at, tokens, at + tokens,
                            at + tokens + batch + 1, at + tokens + 2 * batch + 1, c.stream()));
-    PyObject* r = PyTuple_New(5);
+    PyObject* r = PyTuple_New(7);
     if (!r) throw Refused{};
     PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(slots));
-    for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(r, i + 1, THPVariable_Wrap(o[i]));
+    for (int64_t i = 0, from = 0; i < 4; from += sizes[i++])
+      PyTuple_SET_ITEM(r, i + 1, THPVariable_Wrap(piece(rest, from, sizes[i])));
+    for (int i = 0; i < 2; ++i) {
+      Py_INCREF(a[2 + 3 * i]);  // table, page
+      PyTuple_SET_ITEM(r, 5 + i, a[2 + 3 * i]);
+    }
+    PyObject* args = PyTuple_Pack(1, r);
+    Py_DECREF(r);
+    if (!args) throw Refused{};
+    r = PyTuple_Type.tp_new(g_plan, args, nullptr);
+    Py_DECREF(args);
     return r;
   });
 }
@@ -308,10 +329,17 @@ PyObject* prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// Takes the function that raises for a return code.
-PyObject* set_check(PyObject*, PyObject* f) {
-  Py_INCREF(f);
-  Py_XSETREF(g_check, f);
+// (the function that raises for a return code, the named tuple of a plan)
+PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!count_is(n, 2)) return nullptr;
+  if (!PyType_Check(a[1]) || !PyType_IsSubtype((PyTypeObject*)a[1], &PyTuple_Type)) {
+    PyErr_SetString(PyExc_TypeError, "expected a tuple type");
+    return nullptr;
+  }
+  Py_INCREF(a[0]);
+  Py_XSETREF(g_check, a[0]);
+  Py_INCREF(a[1]);
+  Py_XSETREF(g_plan, (PyTypeObject*)a[1]);
   Py_RETURN_NONE;
 }
 
@@ -319,7 +347,7 @@ PyMethodDef methods[] = {
     {"slots_plan", (PyCFunction)(void (*)())slots_plan, METH_FASTCALL, nullptr},
     {"qk_norm_rope_store", (PyCFunction)(void (*)())qk_norm_rope_store, METH_FASTCALL, nullptr},
     {"prefix_attention", (PyCFunction)(void (*)())prefix_attention, METH_FASTCALL, nullptr},
-    {"set_check", set_check, METH_O, nullptr},
+    {"setup", (PyCFunction)(void (*)())setup, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "gsec_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

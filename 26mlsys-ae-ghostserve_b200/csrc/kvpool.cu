@@ -48,6 +48,7 @@ __global__ void __launch_bounds__(kPlanThreads) slots_plan_kernel(const SlotPlan
   const int tid = threadIdx.x, B = a.batch;
   grid_dep_wait();
   grid_dep_launch();
+  const int64_t cursor = a.cursor[0];
   bool bad = false;
   for (int i = tid; i < B; i += kPlanThreads) {
     int32_t o = a.lens[i], n = a.fresh[i];
@@ -85,11 +86,16 @@ __global__ void __launch_bounds__(kPlanThreads) slots_plan_kernel(const SlotPlan
     wsum[1][tid >> 5] = xp;
   }
   __syncthreads();
-  int64_t bt = xt - st, bp = xp - sp;
-  for (int w = 0; w < (tid >> 5); ++w) {
-    bt += wsum[0][w];
-    bp += wsum[1][w];
+  // sums of the warps before this one: every warp adds them up for itself
+  constexpr int kWarps = kPlanThreads / 32;
+  const int lane = tid & 31, warp = tid >> 5;
+  int64_t vt = lane < warp ? wsum[0][lane % kWarps] : 0, vp = lane < warp ? wsum[1][lane % kWarps] : 0;
+#pragma unroll
+  for (int d = kWarps >> 1; d; d >>= 1) {
+    vt += __shfl_xor_sync(0xffffffffu, vt, d);
+    vp += __shfl_xor_sync(0xffffffffu, vp, d);
   }
+  int64_t bt = xt - st + __shfl_sync(0xffffffffu, vt, 0), bp = xp - sp + __shfl_sync(0xffffffffu, vp, 0);
   for (int i = i0; i < i1; ++i) {
     const int32_t n = cu[i], q = pg[i];
     cu[i] = clamp_i32(bt);
@@ -103,7 +109,6 @@ __global__ void __launch_bounds__(kPlanThreads) slots_plan_kernel(const SlotPlan
   }
   __syncthreads();
   const int32_t total = cu[B], pages = pg[B];
-  const int64_t cursor = a.cursor[0];
   const int64_t gid = (int64_t)blockIdx.x * kPlanThreads + tid, gsize = (int64_t)gridDim.x * kPlanThreads;
   bad |= total > a.capacity;
   const auto take = [&](int64_t k) -> int32_t {  // k-th page of this step
@@ -368,8 +373,8 @@ int launch_store(QkStoreArgs a, cudaStream_t s) {
 
 int slots_plan(const SlotPlanArgs& a, cudaStream_t s) {
   const size_t smem = (3 * (size_t)a.batch + 2) * sizeof(int32_t);
-  const int per_sm = launch_cache().blocks_per_sm(slots_plan_kernel, kPlanThreads, smem);
-  if (per_sm < 0) return check_launch("slots_plan launch shape");
+  if (smem > 32 * 1024 && launch_cache().blocks_per_sm(slots_plan_kernel, kPlanThreads, smem) < 0)
+    return check_launch("slots_plan launch shape");
   // every CTA pays for the sums: no more CTAs than the outputs keep busy
   int64_t grid = (a.capacity / 4 + kPlanThreads - 1) / kPlanThreads;
   if (grid < 1) grid = 1;

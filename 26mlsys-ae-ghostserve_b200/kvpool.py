@@ -40,7 +40,7 @@ def _load():
         spec = importlib.util.spec_from_file_location("gsec_torch", BIND_PATH)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
-        module.set_check(_lib.check)
+        module.setup(_lib.check, SlotPlan)
         _native = module
     return _native
 
@@ -78,8 +78,7 @@ def slots_plan(lens: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free:
     if stream is not None:
         with _on(stream, lens):
             return slots_plan(lens, new, table, free, cursor, page, tokens, base)
-    slots, positions, cu, out, taken = (_native or _load()).slots_plan(lens, new, table, free, cursor, page, tokens, base)
-    return SlotPlan(slots, positions, cu, out, taken, table, page)
+    return (_native or _load()).slots_plan(lens, new, table, free, cursor, page, tokens, base)
 
 
 def qk_norm_rope_store(qkv: torch.Tensor, pool: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor,
