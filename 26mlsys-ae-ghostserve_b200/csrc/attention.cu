@@ -192,7 +192,10 @@ constexpr int kUnitTile = 32, kUnitSegment = 32;
 // per thread; the third warpgroup hands over what it does not need.
 constexpr int kLaunchRegs = 168, kSoftmaxRegs = 200, kOtherRegs = 104;
 static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * kLaunchRegs, "register shares");
-constexpr int kMinShare = 64;       // a stretch is at least about two tiles
+// A stretch is at least half a block's tile. (Four of them, with less to join: one
+// request of 1000 keys on one KV head 14.0 us instead of 11.9, eight of 100 to 600
+// 14.0 instead of 11.9, one of 300 11.3 instead of 11.5.)
+constexpr int kMinShare = 16;
 
 // A block and its keys: rows [blk * kBlock, ...) of the row space that starts at
 // token `tok`; row x of it is token tok + x / group, head kh * group + x % group.
