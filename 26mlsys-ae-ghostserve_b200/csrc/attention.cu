@@ -186,7 +186,9 @@ constexpr int kRows = 128, kKeys = 128, kBlock = 256;
 // that; a segment's beginning and end. (Three quarters and 16: 128 ragged decode
 // requests behind 2047 keys took 205 us instead of 145, 16 behind 32768 60 instead
 // of 50: the blocks of the prefix were late. With segments of 64 and more it is the
-// requests' own keys that are.)
+// requests' own keys that are.) Rows loaded four at a time cost half a block as
+// much as a whole one, and an eighth more is what came out (extends of 64-wide
+// heads 131 -> 124 us).
 constexpr int kUnitTile = 32, kUnitSegment = 32;
 // Registers: a softmax thread holds 64 scores and 64 words of P. The launch has 168
 // per thread; the third warpgroup hands over what it does not need.
@@ -317,7 +319,7 @@ struct Walk {
   __device__ __forceinline__ int slope() const { return g.req < 0 ? 0 : p.slope; }
   __device__ __forceinline__ int units() const {
     const int u = base_units() + slope() * (g.blk + 1);
-    return kUnitSegment + (pair() ? u : u / 2);
+    return kUnitSegment + (pair() ? u : u / 2 + (p.run ? 0 : u / 8));
   }
   __device__ __forceinline__ int units_before(int m) const {
     return (int)((int64_t)m * (kUnitSegment + base_units()) + (int64_t)m * (m + 1) / 2 * slope());
@@ -947,7 +949,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
       // Whole pages as boxes; the rest of a tile, or a tile with a page outside
       // the pool, four rows at a time, with zeros for what is not there (a slot
       // behind the end may hold anything). Only the sixteens that the products
-      // take are loaded.
+      // take are loaded. (Four-row gathers move a tile in about twice a box's time:
+      // 128 ragged decode requests 226 us on pages of one, 126 on pages of 16. By
+      // 16-byte copies of the whole warp it was 311.)
       constexpr int PN = DP / 64;                               // 64-value panels of a row
       constexpr uint32_t kPanel = kRows * 128;
       const int kv = warp - 9, none = (int)a.pool_rows;         // none: a row outside the map
