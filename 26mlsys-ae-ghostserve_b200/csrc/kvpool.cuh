@@ -24,9 +24,6 @@ struct Vec16<__nv_bfloat16> {
       f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
   }
-  static __device__ __forceinline__ float2 unpack2(uint32_t w) {
-    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-  }
   static __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -47,9 +44,6 @@ struct Vec16<__half> {
       f[2 * i] = p.x;
       f[2 * i + 1] = p.y;
     }
-  }
-  static __device__ __forceinline__ float2 unpack2(uint32_t w) {
-    return __half22float2(*reinterpret_cast<const __half2*>(&w));
   }
   static __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);

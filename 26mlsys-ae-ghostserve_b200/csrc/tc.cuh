@@ -1,5 +1,5 @@
 // tc.cuh — the fifth-generation tensor core as PTX: tensor memory, descriptors,
-// matrix instructions and their commits, and 16-byte asynchronous copies.
+// matrix instructions and their commits, tensor copies.
 #pragma once
 
 #include <cuda.h>
@@ -122,15 +122,6 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
 }
 
 // ------------------------------------------------------------------- copies --
-// 16 bytes to shared memory; zeros instead of a read when !valid.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 // Box of a two-dimensional tensor map at (x, y), completing on `bar`.
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
@@ -157,9 +148,6 @@ __device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, 
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
-// Ordinary writes to shared memory before, reads by the tensor core after.
-__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
 // The warpgroup's registers per thread from here on: more only as far as others
 // have given back of what the block was launched with.
 template <int N>
