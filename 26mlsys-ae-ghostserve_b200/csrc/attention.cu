@@ -411,11 +411,12 @@ __device__ __forceinline__ int share(int total, int ctas) {
   return n < kMinShare ? kMinShare : n;
 }
 
-// A wait gives up after 2^24 turns and raises `quit`, which ends every other wait
-// of the CTA.
+// A wait gives up after so many turns (TileShared::turns) and raises `quit`, which
+// ends every other wait of the CTA.
 __device__ __forceinline__ bool long_wait(uint64_t* bar, uint32_t parity, volatile int* quit) {
+  const int turns = quit[1];
 #pragma unroll 1
-  for (int i = 0; i < 1 << 24; ++i) {
+  for (int i = 0; i < turns; ++i) {
     if (pipe::bar_try(bar, parity)) return true;
     if (*quit) return false;
   }
@@ -455,6 +456,7 @@ struct TileShared {
   int total;
   uint32_t tmem;
   int quit;                         // a wait gave up
+  int turns;                        // after so many: more than the CTA's whole stretch can take
   int bad;                          // a page was outside the pool
 };
 static_assert(sizeof(TileShared) <= kBehind, "shared memory behind the tiles");
@@ -659,6 +661,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
     const int x0 = (int)blockIdx.x * share(total, p.ctas);
     if (tid == 0) {
       sh.total = total;
+      // a wait may last as long as a piece; a unit of the line takes 70 ns, a turn 20 and more
+      sh.turns = (1 << 24) + 64 * (share(total, p.ctas) < 1 << 24 ? share(total, p.ctas) : 1 << 24);
       if (x0 < pre) {
         w.prefix();
         sh.first.y = x0;

@@ -148,10 +148,29 @@ int code_of(at::ScalarType t, const char* what) {
   return t == at::kBFloat16 ? GSEC_BF16 : t == at::kHalf ? GSEC_F16 : GSEC_F32;
 }
 
-at::Tensor output(const Call& c, PyObject* o, at::IntArrayRef shape, at::ScalarType type) {
+// The bytes from a tensor's first element to its last.
+struct Span {
+  uintptr_t lo, hi;
+  explicit Span(const at::Tensor& t) : lo((uintptr_t)t.data_ptr()), hi(lo) {
+    if (t.numel() == 0) return;
+    int64_t last = 1;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    hi = lo + last * t.element_size();
+  }
+};
+
+// `out` or a new tensor; not in the memory of what the call reads (or the pool),
+// which other blocks may still be reading when a result is written.
+at::Tensor output(const Call& c, PyObject* o, at::IntArrayRef shape, at::ScalarType type, const at::Tensor& in,
+                  const at::Tensor& pool) {
   if (o == Py_None) return c.empty(shape, type);
   const at::Tensor& t = tensor(o, "out");
   c.flat(t, "out", type);
+  no_grad(t, "out");
+  for (const at::Tensor* x : {&in, &pool}) {
+    const Span a(t), b(*x);
+    NEED(a.hi <= b.lo || b.hi <= a.lo, "out overlaps the call's input or the pool");
+  }
   NEED(t.sizes() == shape, "out must have as many tokens, heads and values as the queries");
   return t;
 }
@@ -259,7 +278,7 @@ PyObject* qk_norm_rope_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int inter = PyObject_IsTrue(a[10]);
     if (inter < 0) throw Refused{};
     NEED(p.heads < (1 << 20) && p.dim < (1 << 20), "pool heads are too many or too wide");
-    at::Tensor out = output(c, a[11], {T, heads, p.dim}, type);
+    at::Tensor out = output(c, a[11], {T, heads, p.dim}, type, qkv, pool);
     const int64_t row = qkv.stride(0) > values ? qkv.stride(0) : values;
     finish(gsec_qk_norm_rope_store(qkv.data_ptr(), row * qkv.element_size(), T, code, heads, (int32_t)p.heads,
                                    (int32_t)p.dim, out.data_ptr(), p.at, p.pitch, p.plane, p.rows, slots.data_ptr(),
@@ -307,7 +326,7 @@ PyObject* prefix_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const double scale = a[8] == Py_None ? 1.0 / std::sqrt((double)(D > 0 ? D : 1)) : real(a[8]);
     const int wants_lse = PyObject_IsTrue(a[10]);
     if (wants_lse < 0) throw Refused{};
-    at::Tensor out = output(c, a[9], {T, hq, D}, type), lse, ws;
+    at::Tensor out = output(c, a[9], {T, hq, D}, type, q, pool), lse, ws;
     if (wants_lse) lse = c.empty({T, hq}, at::kFloat);
     int64_t bytes = 0;
     if (T > 0)

@@ -94,7 +94,8 @@ def qk_norm_rope_store(qkv: torch.Tensor, pool: torch.Tensor, slots: torch.Tenso
     ``2 cos.shape[1]`` values of each then turn by row ``positions[t]`` of ``cos``
     and ``sin`` (fp32 [max_pos, rot / 2]): pairs (i, i + rot/2), or neighbours with
     ``interleaved``. Keys and values go to ``pool[slots[t]]``; a negative slot
-    stores nothing, and no slot may appear twice. Arithmetic in 32 bits, one
+    stores nothing, and no slot may appear twice. ``out`` may overlap neither ``qkv``
+    nor the pool. Arithmetic in 32 bits, one
     rounding. A slot past the pool stores nothing and sets bit 16 of
     ``codec.device_status``; a position outside the tables leaves the row
     unrotated and sets bit 18."""
@@ -116,7 +117,8 @@ def prefix_attention(q: torch.Tensor, pool: torch.Tensor, cu: torch.Tensor, lens
     the ``prefix_len`` keys on the pages ``prefix``, which all requests share, and
     the first ``lens[i] - n + j + 1`` of the request's ``lens[i]`` own keys on its
     row of ``table`` (``lens``, ``cu`` and ``table`` as ``slots_plan`` returns
-    them). ``scale`` defaults to 1 / sqrt(dim). With ``return_lse`` the second
+    them). ``q`` may be strided, but not broadcast; ``out`` may overlap neither ``q``
+    nor the pool. ``scale`` defaults to 1 / sqrt(dim). With ``return_lse`` the second
     result is the log of each row's sum of exponentials, fp32 [tokens, heads]. A
     row that sees no key is 0 with lse -inf; rows from ``cu[-1]`` on are left as
     they were. Keys and values inside a request's length must be finite (a

@@ -330,6 +330,57 @@ def test_prefix_attention_strides():
     check_attention(dict(c, pool=layers[:, 1]))
 
 
+@pytest.mark.parametrize("hq,hk,D", [(8, 8, 128), (4, 2, 64), (12, 4, 128), (24, 4, 64), (7, 1, 128), (40, 2, 64),
+                                     (32, 2, 64), (32, 1, 128), (96, 2, 32), (200, 1, 16)])
+def test_prefix_attention_queries_of_any_group_and_layout(hq, hk, D):
+    """Whole token rows, slices of wider rows, heads first, and a token pitch that is no whole number of heads."""
+    c = attn_case([1, 0, 70, 9], [300, 5, 90, 9], 150, 16, hq, hk, D, HF, seed=hq, pad=2)
+    check_attention(c)
+    T = c["q"].shape[0]
+    for wide in (torch.zeros(T, hq * D + 3 * D, device="cuda", dtype=HF), torch.zeros(T, hq * D + 8, device="cuda", dtype=HF)):
+        part = wide[:, :hq * D].view(T, hq, D)
+        part.copy_(c["q"])
+        check_attention(dict(c, q=part))
+    check_attention(dict(c, q=c["q"].transpose(0, 1).contiguous().transpose(0, 1)))
+    check_attention(dict(attn_case([1], [77], 20, 16, hq, hk, D, BF)))
+
+
+@pytest.mark.parametrize("B,P", [(1000, 0), (1000, 40), (5000, 9)])
+def test_prefix_attention_more_requests_than_threads(B, P):
+    lens = [1 + (i * 7919) % 50 for i in range(B)]
+    q_lens = [i % 3 for i in range(B)]
+    check_attention(attn_case(q_lens, [max(n, m) for n, m in zip(lens, q_lens)], P, 16, 4, 2, 64, BF))
+
+
+def test_prefix_attention_first_scores_far_below():
+    """The first 32 scores of a row are small ones: its reference has to move in the same tile."""
+    c = attn_case([1, 3], [100, 200], 0, 16, 4, 2, 128, BF, garbage=0.0)
+    for i, n in enumerate((100, 200)):
+        pages = c["table"][i, :-(-n // 16)].long()
+        slots = (pages[:, None] * 16 + torch.arange(16, device="cuda")).reshape(-1)[:n]
+        c["pool"][slots[:40], 0] *= 0.01
+        c["pool"][slots[40:], 0] *= 6
+    check_attention(c)
+
+
+def test_out_may_not_overlap():
+    c = attn_case([1, 2], [20, 30], 16, 16, 4, 2, 64, BF)
+    room = torch.zeros(5, 4, 64, device="cuda", dtype=BF)
+    room[:3] = c["q"]
+    for q, out in ((c["q"], c["q"]), (room[:3], room[2:])):
+        with pytest.raises(ValueError, match="overlaps"):
+            kv().prefix_attention(**dict(c, q=q), out=out)
+    with pytest.raises(ValueError, match="overlaps"):
+        kv().prefix_attention(**c, out=c["pool"].view(-1)[:3 * 4 * 64].view(3, 4, 64))
+    with pytest.raises(ValueError, match="gradient"):
+        kv().prefix_attention(**c, out=torch.zeros(3, 4, 64, device="cuda", dtype=BF, requires_grad=True))
+    with pytest.raises(ValueError, match="stride"):
+        kv().prefix_attention(**dict(c, q=c["q"][:, :1].expand(-1, 4, -1)))
+    qkv, pool, slots, positions, cos, sin, w = store_case(9, 4, 2, 64, 64, BF, True)
+    with pytest.raises(ValueError, match="overlaps"):
+        kv().qk_norm_rope_store(qkv, pool, slots, positions, cos, sin, 4, out=qkv.view(-1)[:9 * 256].view(9, 4, 64))
+
+
 def test_prefix_attention_far_slots():
     """Pages more than 2^32 bytes into the pool."""
     c = attn_case([1, 20], [70, 40], 300, 16, 8, 8, 128, BF)

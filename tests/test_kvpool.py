@@ -70,6 +70,7 @@ def test_qk_norm_rope_store_refusals(bad, match):
     (dict(cu=None), "null"), (dict(lens=None), "null"), (dict(prefix_len=5), "null"), (dict(table=None), "table"),
     (dict(pitch=7), "table"), (dict(page=0), "page"), (dict(prefix=A[7], prefix_len=1 << 30), "2\\^30"),
     (dict(prefix=A[7], prefix_len=-1), "keys"), (dict(q_head=264), "aligned"), (dict(q=P(0x10008)), "aligned"),
+    (dict(q_head=0), "strides"), (dict(q_pitch=0), "strides"), (dict(q_pitch=1 << 40), "strides"),
     (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(ws=None), "workspace"),
     (dict(ws_bytes=16), "workspace"), (dict(ws=P(0x70008)), "workspace"),
 ])
