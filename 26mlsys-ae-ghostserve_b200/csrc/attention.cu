@@ -26,22 +26,30 @@ __device__ __forceinline__ int64_t key_slot(const AttnArgs& a, int r, int32_t x)
   return page < 0 || slot >= a.pool_rows ? -1 : slot;
 }
 
-// ------------------------------------------------------ one row per CTA -------
-// One query row per CTA. The keys are dealt out to lane groups (a group holds
-// one key's vector per step), each with its own running maximum m, sum l and
-// accumulator; they meet at the end by
+// ---------------------------------------------------- a few rows per CTA -------
+// What the tensor core does not take: G query heads of one token that share a KV
+// head per CTA, so that a key is read once for them. The keys are dealt out to lane
+// groups (a group holds one key's vector per step), each with its own running
+// maximum m, sum l and accumulator per head; they meet at the end by
 //   m = max m_g, l = sum l_g 2^(m_g - m), o = sum o_g 2^(m_g - m) / l.
+// Bound by the latency of a step (lookup, loads, sum over the lanes), of which each
+// has several keys: 16 requests of 32 fp32 heads on 8 KV heads of 128, behind 4096
+// keys, 367 us; 256-wide bf16 heads 329. (One head per CTA and a key a step: 715 and
+// 825; G = 2: 400 and 337.) Not split over long keys: few rows behind a long
+// cache leave SMs idle.
 constexpr int kRowThreads = 256;
 
-template <typename T, int NC>
+template <typename T, int NC, int G>
 __global__ void __launch_bounds__(kRowThreads) attend_row_kernel(const AttnArgs a, int L) {
   using V = Vec16<T>;
   constexpr int E = V::N * NC;
-  extern __shared__ float sm[];  // [groups][dim + 2]
+  extern __shared__ float sm[];  // [lane groups][G][dim + 2]
   grid_dep_wait();
   grid_dep_launch();
-  const int64_t t = blockIdx.x / a.hq;
-  const int h = (int)(blockIdx.x - t * a.hq), kh = (int)a.group_div.div(h);
+  const int parts = (a.group + G - 1) / G;                // CTAs of a token and KV head
+  const int64_t t = blockIdx.x / (unsigned)(a.hk * parts);
+  const int rest = (int)(blockIdx.x - t * (a.hk * parts)), kh = rest / parts, g0 = (rest - kh * parts) * G;
+  const int h0 = kh * a.group + g0, nh = a.group - g0 < G ? a.group - g0 : G;
   const int total = a.cu[a.batch] < a.tokens ? a.cu[a.batch] : (int)a.tokens;
   if (t >= total) return;  // rows behind the last request stay as they are
   // the request of token t: the last r with cu[r] <= t
@@ -64,85 +72,142 @@ __global__ void __launch_bounds__(kRowThreads) attend_row_kernel(const AttnArgs 
   const int lane = threadIdx.x % L, grp = threadIdx.x / L, ngrp = kRowThreads / L;
   const int vecs = a.dim / V::N;
   const float scale = a.scale * 1.4426950408889634f;
-  float q[E], o[E], m = -INFINITY, l = 0.f;
+  float q[G][E], o[G][E], m[G], l[G];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int v = lane + c * L;
-    uint4 w = vzero();
-    if (v < vecs) w = *reinterpret_cast<const uint4*>(a.q + t * a.q_pitch + h * a.q_head + v * 16);
-    V::unpack(w, q + c * V::N);
-  }
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] *= scale;
-    o[e] = 0.f;
-  }
-  const int rounds = (keys + ngrp - 1) / ngrp;
-  for (int it = 0; it < rounds; ++it) {
-    const int32_t x = it * ngrp + grp;
-    const int64_t slot = x < keys ? key_slot(a, r, x) : -1;
-    if (x < keys && slot < 0) atomicOr(&g_attn_status, 1u);
-    const char* rec = a.pool + slot * a.pitch + (int64_t)kh * a.dim * sizeof(T);
-    float k[E], v[E], s = 0.f;
+  for (int h = 0; h < G; ++h) {
+    m[h] = -INFINITY;
+    l[h] = 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int i = lane + c * L;
-      uint4 kw = vzero(), vw = vzero();
-      if (slot >= 0 && i < vecs) {
-        kw = __ldg(reinterpret_cast<const uint4*>(rec) + i);
-        vw = __ldg(reinterpret_cast<const uint4*>(rec + a.plane) + i);
-      }
-      V::unpack(kw, k + c * V::N);
-      V::unpack(vw, v + c * V::N);
+      const int v = lane + c * L;
+      uint4 w = vzero();
+      if (v < vecs && h < nh) w = *reinterpret_cast<const uint4*>(a.q + t * a.q_pitch + (h0 + h) * a.q_head + v * 16);
+      V::unpack(w, q[h] + c * V::N);
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) s += q[e] * k[e];
-    for (int d = L >> 1; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    if (x < keys) {
-      const float top = fmaxf(m, s);
-      const float old = top == -INFINITY ? 1.f : exp2f(m - top);  // both empty: nothing to scale
-      const float p = top == -INFINITY ? 0.f : exp2f(s - top);
-      l = l * old + p;
+    for (int e = 0; e < E; ++e) {
+      q[h][e] *= scale;
+      o[h][e] = 0.f;
+    }
+  }
+  // kAhead keys' vectors are on their way at a time
+  constexpr int kAhead = NC == 1 ? 4 : 2;
+  const int rounds = (keys + ngrp - 1) / ngrp;
+  for (int it = 0; it < rounds; it += kAhead) {
+    uint4 kw[kAhead][NC], vw[kAhead][NC];
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = o[e] * old + p * v[e];
-      m = top;
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t x = (int64_t)(it + u) * ngrp + grp;
+      const int64_t slot = x < keys ? key_slot(a, r, (int32_t)x) : -1;
+      if (x < keys && slot < 0) atomicOr(&g_attn_status, 1u);
+      const char* rec = a.pool + slot * a.pitch + (int64_t)kh * a.dim * sizeof(T);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int i = lane + c * L;
+        const bool is = slot >= 0 && i < vecs;
+        kw[u][c] = is ? __ldg(reinterpret_cast<const uint4*>(rec) + i) : vzero();
+        vw[u][c] = is ? __ldg(reinterpret_cast<const uint4*>(rec + a.plane) + i) : vzero();
+      }
+    }
+    float s[kAhead][G];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      float k[E];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) V::unpack(kw[u][c], k + c * V::N);
+#pragma unroll
+      for (int h = 0; h < G; ++h) {
+        s[u][h] = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) s[u][h] += q[h][e] * k[e];
+      }
+    }
+    for (int d = L >> 1; d; d >>= 1) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+        for (int h = 0; h < G; ++h) s[u][h] += __shfl_xor_sync(0xffffffffu, s[u][h], d);
+    }
+#pragma unroll
+    for (int h = 0; h < G; ++h) {
+      float top = m[h];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if ((int64_t)(it + u) * ngrp + grp >= keys) s[u][h] = -INFINITY;
+        top = fmaxf(top, s[u][h]);
+      }
+      const float old = top == -INFINITY ? 1.f : exp2f(m[h] - top);  // all empty: nothing to scale
+      m[h] = top;
+      l[h] *= old;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[h][e] *= old;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        s[u][h] = s[u][h] == -INFINITY ? 0.f : exp2f(s[u][h] - top);
+        l[h] += s[u][h];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      float v[E];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) V::unpack(vw[u][c], v + c * V::N);
+#pragma unroll
+      for (int h = 0; h < G; ++h)
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[h][e] += s[u][h] * v[e];
     }
   }
   // the groups meet in shared memory
-  float* mine = sm + grp * (a.dim + 2);
-  if (lane == 0) {
-    mine[a.dim] = m;
-    mine[a.dim + 1] = l;
+#pragma unroll
+  for (int h = 0; h < G; ++h) {
+    float* mine = sm + (grp * G + h) * (a.dim + 2);
+    if (lane == 0) {
+      mine[a.dim] = m[h];
+      mine[a.dim + 1] = l[h];
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < V::N; ++e)
+        if (lane + c * L < vecs) mine[(lane + c * L) * V::N + e] = o[h][c * V::N + e];
   }
-#pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int e = 0; e < V::N; ++e)
-      if (lane + c * L < vecs) mine[(lane + c * L) * V::N + e] = o[c * V::N + e];
   __syncthreads();
-  float top = -INFINITY, sum = 0.f;
-  for (int g = 0; g < ngrp; ++g) top = fmaxf(top, sm[g * (a.dim + 2) + a.dim]);
-  for (int g = 0; g < ngrp; ++g)
-    if (sm[g * (a.dim + 2) + a.dim] > -INFINITY)
-      sum += sm[g * (a.dim + 2) + a.dim + 1] * exp2f(sm[g * (a.dim + 2) + a.dim] - top);
-  for (int d = threadIdx.x; d < a.dim; d += kRowThreads) {
-    float x = 0.f;
+  for (int h = 0; h < nh; ++h) {
+    const float* at = sm + h * (a.dim + 2);
+    const int step = G * (a.dim + 2);
+    float top = -INFINITY, sum = 0.f;
+    for (int g = 0; g < ngrp; ++g) top = fmaxf(top, at[g * step + a.dim]);
     for (int g = 0; g < ngrp; ++g)
-      if (sm[g * (a.dim + 2) + a.dim] > -INFINITY)
-        x += sm[g * (a.dim + 2) + d] * exp2f(sm[g * (a.dim + 2) + a.dim] - top);
-    reinterpret_cast<T*>(a.out)[(t * a.hq + h) * a.dim + d] = (T)(sum == 0.f ? 0.f : x / sum);
+      if (at[g * step + a.dim] > -INFINITY) sum += at[g * step + a.dim + 1] * exp2f(at[g * step + a.dim] - top);
+    const int64_t row = t * a.hq + h0 + h;
+    for (int d = threadIdx.x; d < a.dim; d += kRowThreads) {
+      float x = 0.f;
+      for (int g = 0; g < ngrp; ++g)
+        if (at[g * step + a.dim] > -INFINITY) x += at[g * step + d] * exp2f(at[g * step + a.dim] - top);
+      reinterpret_cast<T*>(a.out)[row * a.dim + d] = (T)(sum == 0.f ? 0.f : x / sum);
+    }
+    if (threadIdx.x == 0 && a.lse) a.lse[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
   }
-  if (threadIdx.x == 0 && a.lse) a.lse[t * a.hq + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
+template <typename T, int NC, int G>
+int launch_rows(const AttnArgs& a, int L, cudaStream_t s) {
+  const size_t smem = (size_t)(kRowThreads / L) * G * (a.dim + 2) * sizeof(float);
+  if (launch_cache().blocks_per_sm(attend_row_kernel<T, NC, G>, kRowThreads, smem) < 0)
+    return check_launch("attend_row launch shape");
+  const int64_t grid = a.tokens * a.hk * ((a.group + G - 1) / G);  // at most tokens * hq
+  return launch_rc(launch_pdl(attend_row_kernel<T, NC, G>, dim3((unsigned)grid), dim3(kRowThreads), smem, s, a, L),
+                   "prefix_attention");
+}
+
+// Heads together as long as half of the SMs are busy.
 template <typename T, int NC>
 int launch_rows(const AttnArgs& a, int L, cudaStream_t s) {
-  const size_t smem = (size_t)(kRowThreads / L) * (a.dim + 2) * sizeof(float);
-  if (launch_cache().blocks_per_sm(attend_row_kernel<T, NC>, kRowThreads, smem) < 0)
-    return check_launch("attend_row launch shape");
-  return launch_rc(launch_pdl(attend_row_kernel<T, NC>, dim3((unsigned)(a.tokens * a.hq)), dim3(kRowThreads), smem, s,
-                              a, L),
-                   "prefix_attention");
+  const int64_t heads = a.tokens * a.hk;
+  if (a.group >= 4 && heads * ((a.group + 3) / 4) * 2 >= sm_count()) return launch_rows<T, NC, 4>(a, L, s);
+  if (a.group >= 2 && heads * ((a.group + 1) / 2) * 2 >= sm_count()) return launch_rows<T, NC, 2>(a, L, s);
+  return launch_rows<T, NC, 1>(a, L, s);
 }
 
 template <typename T>
@@ -180,6 +245,12 @@ int attend_rows(const AttnArgs& a, cudaStream_t s) {
 // line is one warp's work, which hands the pieces to the others through shared
 // memory, and loops are unrolled only as far as they have to be (with the walk in
 // every role and 128-column bodies a one-tile segment took 12000 cycles).
+// Measured (bf16, 32 heads on 8 KV heads of 128, pages of 16): 16 decode requests
+// behind 32768 keys 43 us, 3.7 TB/s; 128 ragged ones behind 2047 150 us, 4.4 TB/s;
+// 256 behind 24576 180 us, 576 TFLOP/s; a 2048-token chunk behind 30720 1140 us, 940
+// TFLOP/s, power capped (990 us alone). The first two are bound by DRAM and the
+// beginnings and ends of segments, the others by a step's chain: scores, softmax
+// (1700 cycles), sums, and only then the next scores, in the same tensor memory.
 constexpr int kTileThreads = 384;   // 2 softmax warpgroups; a warp each issues products, loads K, loads V, walks and loads Q
 constexpr int kRows = 128, kKeys = 128, kBlock = 256;
 // Units of the line: a tile of a whole block, half a block's tile being half of
@@ -846,8 +917,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
       // -------------------------------------------------------- products ----
       // One thread. Step s runs on S, P and O number s & 1; its scores are issued
       // right after the P V of step s - 2. A lone thread takes five cycles and more
-      // for an instruction, so what can be done before P arrives is, and the
-      // products are unrolled.
+      // for an instruction, so what can be done before P arrives is. (The scores'
+      // products in a loop: a 2048-token chunk 1205 us instead of 1140. The sums' are:
+      // unrolled 256 requests on one prefix took 183 us instead of 180.)
       if (tc::elect()) {
         const uint32_t id_s = tc::idesc(Vec16<T>::bf16, kRows, 0, false, a.scale < 0.f);
         const uint32_t id_o = tc::idesc(Vec16<T>::bf16, kRows, a.dim, true);
@@ -1221,6 +1293,9 @@ __device__ __forceinline__ void write_row(const AttnArgs& a, int64_t grow, const
   if (lane == 0 && a.lse) a.lse[grow] = s.l == 0.f ? -INFINITY : (s.m + log2f(s.l)) * 0.6931471805599453f;
 }
 
+// Bound by latency: about 4 us behind the tiles, 12 to 17 us with thousands of cut
+// rows and a cold cache.
+//
 // Rows with one segment each (prefix and own keys in one, or no prefix): only
 // those of cut segments. Block (c, i) does the share i of the rows of the cut
 // segment that ends in CTA c's stretch.

@@ -274,6 +274,13 @@ def test_prefix_attention_fp32_and_wide_heads():
     check_attention(attn_case([2, 1], [40, 131], 65, 16, 4, 2, 8, HF))
 
 
+@pytest.mark.parametrize("dtype,hq,hk,D", [(F4, 8, 1, 128), (F4, 10, 2, 64), (BF, 12, 4, 256), (HF, 6, 1, 136), (F4, 3, 3, 4),
+                                           (BF, 8, 2, 8), (F4, 14, 2, 252)])
+def test_prefix_attention_rows_of_few_and_many_tokens(dtype, hq, hk, D):
+    check_attention(attn_case([1, 2, 0], [40, 131, 3], 65, 16, hq, hk, D, dtype))
+    check_attention(attn_case([170, 1, 3], [170, 300, 0], 33, 16, hq, hk, D, dtype, pad=2))
+
+
 def test_prefix_attention_empty_rows():
     # no keys at all; more queries than own keys (the first see nothing, or the prefix alone)
     c = attn_case([2, 1, 6], [0, 0, 4], 0, 16, 4, 2, 64, BF)
