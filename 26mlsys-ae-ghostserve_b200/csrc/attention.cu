@@ -482,7 +482,7 @@ __device__ __forceinline__ int share(int total, int ctas) {
   return n < kMinShare ? kMinShare : n;
 }
 
-// A wait gives up after so many turns (TileShared::turns) and raises `quit`, which
+// A wait gives up after so many turns (TileShared::quit) and raises `quit`, which
 // ends every other wait of the CTA.
 __device__ __forceinline__ bool long_wait(uint64_t* bar, uint32_t parity, volatile int* quit) {
   const int turns = quit[1];
@@ -526,8 +526,7 @@ struct TileShared {
   Start first;                      // where this CTA's stretch starts
   int total;
   uint32_t tmem;
-  int quit;                         // a wait gave up
-  int turns;                        // after so many: more than the CTA's whole stretch can take
+  int quit[2];                      // a wait gave up; after so many turns: more than the CTA's stretch can take
   int bad;                          // a page was outside the pool
 };
 static_assert(sizeof(TileShared) <= kBehind, "shared memory behind the tiles");
@@ -683,7 +682,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
     pipe::bar_init(&sh.handed, 4);
     pipe::bar_init(&sh.taken, 4);
     pipe::bar_init_fence();
-    sh.quit = (tc::smem_addr(smem) & 1023u) != 0;  // the swizzle counts from 1024-byte patterns
+    sh.quit[0] = (tc::smem_addr(smem) & 1023u) != 0;  // the swizzle counts from 1024-byte patterns
     sh.bad = 0;
   }
   if (warp == 8) {
@@ -733,7 +732,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
     if (tid == 0) {
       sh.total = total;
       // a wait may last as long as a piece; a unit of the line takes 70 ns, a turn 20 and more
-      sh.turns = (1 << 24) + 64 * (share(total, p.ctas) < 1 << 24 ? share(total, p.ctas) : 1 << 24);
+      sh.quit[1] = (1 << 24) + 64 * (share(total, p.ctas) < 1 << 24 ? share(total, p.ctas) : 1 << 24);
       if (x0 < pre) {
         w.prefix();
         sh.first.y = x0;
@@ -764,7 +763,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
   const uint32_t tmem = sh.tmem;
   const int unit = share(sh.total, p.ctas);
   const int x0 = (int)blockIdx.x * unit, x1 = sh.total - x0 < unit ? sh.total : x0 + unit;
-  volatile int* quit = &sh.quit;
+  volatile int* quit = sh.quit;
   const float c = fabsf(a.scale) * 1.4426950408889634f;
   if (x0 < x1 && !*quit) {
     // Reads piece number `i` of the CTA; whoever has read it says so with done_piece.
@@ -1219,7 +1218,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
   __syncthreads();
   tc::fence_after();
   if (warp == 8) tc::dealloc(tmem, 512);
-  if (tid == 0 && (sh.quit || sh.bad)) atomicOr(&g_attn_status, (sh.quit ? 2u : 0u) | (sh.bad ? 1u : 0u));
+  if (tid == 0 && (sh.quit[0] || sh.bad)) atomicOr(&g_attn_status, (sh.quit[0] ? 2u : 0u) | (sh.bad ? 1u : 0u));
 }
 
 // ------------------------------------------------------------ joining parts ---

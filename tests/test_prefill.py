@@ -95,6 +95,6 @@ def test_pool_attention_is_refused_where_it_cannot_run():
     with pytest.raises(ValueError, match="CUDA"):
         pre.TPPrefill(spec, 32, "cpu", attention="pool")
     with pytest.raises(ValueError, match="attention"):
-        pre.TPPrefill(spec, 32, "cpu", attention="flash")
+        pre.TPPrefill(spec, 32, "cpu", attention="other")
     with pytest.raises(ValueError, match="pool"):
         pre.TPPrefill(spec, 32, "cpu").extend(torch.arange(4), None)
