@@ -1055,21 +1055,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
             if (lane < boxes) rows[lane] = y;
           }
           const int quad0 = (boxes << p.run_log) >> 2, quads = sixteens(valid) * 4;
-          if (lane >= quad0 && lane < quads) {
-            int32_t* z = rows + lane * 4;                       // behind the boxes' entries
-            const auto look = [&](int j) {
-              const bool is = lane * 4 + j < valid;
-              const int64_t sl = is ? key_slot(a, g.req, k0 + lane * 4 + j) : -1;
-              if (is && sl < 0) sh.bad = 1;
-              z[j] = sl < 0 ? none : (int32_t)sl;
-            };
-            if (ROWS) {                                         // four lookups in flight
+          const auto look = [&](int k) {                        // rows behind the boxes' entries
+            const bool is = k < valid;
+            const int64_t sl = is ? key_slot(a, g.req, k0 + k) : -1;
+            if (is && sl < 0) sh.bad = 1;
+            rows[k] = sl < 0 ? none : (int32_t)sl;
+          };
+          if (ROWS) {                                           // every tile: four lookups in flight
+            if (lane < quads) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) look(j);
-            } else {
-#pragma unroll 1
-              for (int j = 0; j < 4; ++j) look(j);
+              for (int j = 0; j < 4; ++j) look(lane * 4 + j);
             }
+          } else {                                              // a tail, mostly less than 32 rows: little code
+#pragma unroll 1
+            for (int k = quad0 * 4 + lane; k < quads * 4; k += 32) look(k);
           }
           const uint32_t st = stage0 + pos % turns;
           __syncwarp();
