@@ -178,13 +178,16 @@ __global__ void __launch_bounds__(kRowThreads) attend_row_kernel(const AttnArgs 
     const int step = G * (a.dim + 2);
     float top = -INFINITY, sum = 0.f;
     for (int g = 0; g < ngrp; ++g) top = fmaxf(top, at[g * step + a.dim]);
-    for (int g = 0; g < ngrp; ++g)
-      if (at[g * step + a.dim] > -INFINITY) sum += at[g * step + a.dim + 1] * exp2f(at[g * step + a.dim] - top);
+    // a group without a maximum has l = o = 0, or they are not numbers (a maximum passes those over) and stay so
+    const auto weight = [&](int g) {
+      const float mg = at[g * step + a.dim];
+      return mg == -INFINITY ? 1.f : exp2f(mg - top);
+    };
+    for (int g = 0; g < ngrp; ++g) sum += at[g * step + a.dim + 1] * weight(g);
     const int64_t row = t * a.hq + h0 + h;
     for (int d = threadIdx.x; d < a.dim; d += kRowThreads) {
       float x = 0.f;
-      for (int g = 0; g < ngrp; ++g)
-        if (at[g * step + a.dim] > -INFINITY) x += at[g * step + d] * exp2f(at[g * step + a.dim] - top);
+      for (int g = 0; g < ngrp; ++g) x += at[g * step + d] * weight(g);
       reinterpret_cast<T*>(a.out)[row * a.dim + d] = (T)(sum == 0.f ? 0.f : x / sum);
     }
     if (threadIdx.x == 0 && a.lse) a.lse[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;

@@ -1,0 +1,85 @@
+"""KV-pool serving operators at the calls that the main tests leave out."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import kvpool_ref as ref
+from conftest import pkg
+from test_gpu_kvpool import BF, F4, HF, attn_case, kv
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def device_status_clean():
+    """Tests that flag something on purpose clear it themselves."""
+    yield
+    assert pkg("codec").device_status(clear=True) == 0
+
+
+def check_rows(o, lse, c, on, **kw):
+    """The rows `on` [tokens, heads] of (o, lse) against the plain form."""
+    want, wl, to, tl = ref.attention(**c, **kw)
+    off = ((o.double() - want).abs() <= to).all(-1) | ~on
+    assert bool(off.all())
+    empty = wl == -math.inf
+    assert bool((((lse.double() - wl).abs() <= tl) | empty | ~on).all())
+    assert bool(((lse == -math.inf) == empty)[on].all())
+
+
+# ---------------------------------------------------------- not a number ------
+ROWS_AND_TILES = [(F4, 8, 2, 64), (F4, 1, 1, 4), (BF, 4, 2, 256), (HF, 6, 1, 136), (BF, 8, 2, 8), (BF, 8, 2, 128),
+                  (HF, 6, 2, 64)]
+
+
+@pytest.mark.parametrize("dtype,hq,hk,D", ROWS_AND_TILES)
+@pytest.mark.parametrize("q_lens,lens,P", [([1], [1], 0), ([1, 3, 0, 20], [7, 300, 5, 20], 0),
+                                           ([1, 1, 1, 1, 40], [5, 1, 128, 257, 300], 385)])
+def test_a_query_that_is_not_a_number_stays_so(dtype, hq, hk, D, q_lens, lens, P):
+    """All values of one head, or one value of another: the row is not a number throughout, its neighbours are as
+    without it."""
+    c = attn_case(q_lens, lens, P, 16, hq, hk, D, dtype)
+    T = c["q"].shape[0]
+    bad = torch.zeros(T, hq, dtype=torch.bool, device="cuda")
+    bad[T - 1, 0] = bad[T // 2, hq - 1] = True
+    q = c["q"].clone()
+    q[T // 2, hq - 1, D // 2] = math.nan
+    q[T - 1, 0] = math.nan
+    o, lse = kv().prefix_attention(**dict(c, q=q), return_lse=True)
+    assert bool(torch.isnan(o[bad]).all()) and bool(torch.isnan(lse[bad]).all())
+    check_rows(o, lse, c, ~bad)
+
+
+@pytest.mark.parametrize("dtype,hq,hk,D", ROWS_AND_TILES)
+def test_a_key_or_value_that_is_not_a_number_shows(dtype, hq, hk, D):
+    """Every row that sees the key is not a number; a value spoils its own column. Other requests and other KV heads
+    are as without it."""
+    c = attn_case([1, 2, 1], [3, 40, 200], 0, 16, hq, hk, D, dtype, garbage=0.0)
+    group = hq // hk
+    slot = int(c["table"][2, 4]) * 16 + 5
+    on = torch.ones(4, hq, dtype=torch.bool, device="cuda")
+    on[3, :group] = False
+    pool = c["pool"].clone()
+    pool[slot, 0, 0, D - 1] = math.nan
+    o, lse = kv().prefix_attention(**dict(c, pool=pool), return_lse=True)
+    assert bool(torch.isnan(o[~on]).all()) and bool(torch.isnan(lse[~on]).all())
+    check_rows(o, lse, c, on)
+    pool = c["pool"].clone()
+    pool[slot, 1, 0, D - 1] = math.nan
+    o, lse = kv().prefix_attention(**dict(c, pool=pool), return_lse=True)
+    assert bool(torch.isnan(o[3, :group, D - 1]).all()) and not bool(torch.isnan(o[3, :group, :D - 1]).any())
+    check_rows(o, lse, c, on)
+
+
+def test_a_scale_next_to_nothing_keeps_what_is_not_a_number():
+    c = attn_case([1, 20], [70, 20], 40, 16, 4, 2, 64, BF)
+    q = c["q"].clone()
+    q[3, 1] = math.nan
+    o, lse = kv().prefix_attention(**dict(c, q=q), scale=1e-30, return_lse=True)
+    on = torch.ones(21, 4, dtype=torch.bool, device="cuda")
+    on[3, 1] = False
+    assert bool(torch.isnan(o[~on]).all()) and bool(torch.isnan(lse[~on]).all())
+    check_rows(o, lse, c, on, scale=1e-30)
