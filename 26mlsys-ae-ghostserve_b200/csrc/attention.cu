@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(kRowThreads) attend_row_kernel(const AttnArgs 
   const int rest = (int)(blockIdx.x - t * (a.hk * parts)), kh = rest / parts, g0 = (rest - kh * parts) * G;
   const int h0 = kh * a.group + g0, nh = a.group - g0 < G ? a.group - g0 : G;
   const int total = a.cu[a.batch] < a.tokens ? a.cu[a.batch] : (int)a.tokens;
-  if (t >= total) return;  // rows behind the last request stay as they are
+  if (t >= total || t < a.cu[0]) return;  // rows outside the requests stay as they are
   // the request of token t: the last r with cu[r] <= t
   int r = 0, hi = a.batch;
   while (hi - r > 1) {
@@ -329,12 +329,17 @@ __device__ __forceinline__ int live_tokens(const AttnArgs& a) {
   const int n = __ldg(a.cu + a.batch);
   return n < 0 ? 0 : (n > a.tokens ? (int)a.tokens : n);
 }
+// The first request's first token: not 0 where a call takes a part of a batch.
+__device__ __forceinline__ int first_token(const AttnArgs& a) {
+  const int n = __ldg(a.cu);
+  return n < 0 ? 0 : n;
+}
 
 // The line as a thread walks it.
 struct Walk {
   const AttnArgs& a;
   const TilePlan& p;
-  int live;              // query tokens of the batch
+  int live;              // where the batch's query tokens end
   Segment g;
   __device__ __forceinline__ Walk(const AttnArgs& a_, const TilePlan& p_, int live_) : a(a_), p(p_), live(live_) {}
 
@@ -357,8 +362,8 @@ struct Walk {
   }
   __device__ __forceinline__ void prefix() {
     g.req = -1;
-    g.tok = 0;
-    g.ntok = live;
+    g.tok = first_token(a);
+    g.ntok = live > g.tok ? live - g.tok : 0;
     g.len = 0;
     g.nblk = blocks();
   }
@@ -1330,7 +1335,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttnArgs a, cons
   grid_dep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % W;
   const int64_t grow = (int64_t)blockIdx.x * (8 / W) + warp / W, all = a.tokens * a.hq;
-  const bool on = grow < (int64_t)live_tokens(a) * a.hq;
+  const bool on = grow >= (int64_t)first_token(a) * a.hq && grow < (int64_t)live_tokens(a) * a.hq;
   Sum sum;
   if (on) {
     const int2 at[2] = {__ldg(p.place + grow), __ldg(p.place + all + grow)};
@@ -1341,7 +1346,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttnArgs a, cons
       if (at[u].x < 0) {
         if (k0 == 0) sum.add(row4(p.whole + (u * all + grow) * a.dim, a.dim, lane), __ldg(p.whole_lse + u * all + grow));
       } else {
-        // (a token that the batch's offsets leave out has no place: what is read stays inside the workspace)
+        // (a token that offsets out of order leave out has no place: what is read stays inside the workspace)
         const int c0 = (at[u].x & 0xffff) < p.ctas ? at[u].x & 0xffff : 0, c1 = at[u].y < p.ctas ? at[u].y : 0;
         add_cuts(sum, p, a.dim, c0, c1, (at[u].x >> 16) & (kBlock - 1), k0, W, lane);
       }

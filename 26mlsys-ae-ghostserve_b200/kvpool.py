@@ -117,13 +117,14 @@ def prefix_attention(q: torch.Tensor, pool: torch.Tensor, cu: torch.Tensor, lens
     the ``prefix_len`` keys on the pages ``prefix``, which all requests share, and
     the first ``lens[i] - n + j + 1`` of the request's ``lens[i]`` own keys on its
     row of ``table`` (``lens``, ``cu`` and ``table`` as ``slots_plan`` returns
-    them). ``q`` may be strided, but not broadcast; ``out`` may overlap neither ``q``
-    nor the pool. ``scale`` defaults to 1 / sqrt(dim). With ``return_lse`` the second
-    result is the log of each row's sum of exponentials, fp32 [tokens, heads]. A
-    row that sees no key is 0 with lse -inf; rows from ``cu[-1]`` on are left as
-    they were. Keys and values inside a request's length must be finite (a
-    non-finite value may spread to earlier tokens of the same request); slots outside
-    all lengths may hold anything. A page outside the pool reads as zeros and a
+    them, or slices of those for a part of a batch). ``q`` may be strided, but not
+    broadcast; ``out`` may overlap neither ``q`` nor the pool. ``scale`` defaults to
+    1 / sqrt(dim). With ``return_lse`` the second result is the log of each row's sum
+    of exponentials, fp32 [tokens, heads]. A row that sees no key is 0 with lse -inf;
+    rows before ``cu[0]`` and from ``cu[-1]`` on are left as they were. Keys and
+    values inside a request's length must be finite (a non-finite value may spread to
+    earlier tokens of the same request); slots outside all lengths may hold anything.
+    A page outside the pool reads as zeros and a
     length past the table is cut; both set bit 19 of ``codec.device_status``."""
     if stream is not None:
         with _on(stream, q):

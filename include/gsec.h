@@ -209,8 +209,8 @@ GSEC_API int gsec_qk_norm_rope_store(const void* qkv, int64_t qkv_pitch, int64_t
  * on the pages `prefix` and to the request's own keys (lens[i], on its row of
  * `table`): token j sees own keys 0 .. lens[i] - n + j. hq / hk query heads read
  * each KV head. out ([tokens, hq, dim]) and lse ([tokens, hq], natural log, may
- * be null); a row that sees no key is 0 and -inf, rows from cu[batch] on are not
- * written. q: byte strides q_pitch (token) and q_head (head), at least a head's
+ * be null); a row that sees no key is 0 and -inf, rows before cu[0] and from
+ * cu[batch] on are not written. q: byte strides q_pitch (token) and q_head (head), at least a head's
  * bytes each (no broadcast). dim: whole 16-byte
  * vectors, at most 256 values. Own and prefix keys and values that a row does not
  * see must be finite where another row of the same request sees them; slots

@@ -83,3 +83,27 @@ def test_a_scale_next_to_nothing_keeps_what_is_not_a_number():
     on[3, 1] = False
     assert bool(torch.isnan(o[~on]).all()) and bool(torch.isnan(lse[~on]).all())
     check_rows(o, lse, c, on, scale=1e-30)
+
+
+# ------------------------------------------------------- parts of a batch -----
+@pytest.mark.parametrize("dtype,hq,hk,D", [(BF, 8, 2, 128), (HF, 4, 4, 64), (F4, 4, 2, 64), (BF, 4, 2, 256)])
+@pytest.mark.parametrize("P", [0, 150, 2000])
+@pytest.mark.parametrize("q_lens,lens", [([1, 4, 2, 0, 1, 3], [9, 30, 70, 4, 20, 33]),
+                                         ([130, 1, 140, 300], [200, 5, 140, 301])])
+def test_parts_of_a_batch_share_queries_and_out(dtype, hq, hk, D, P, q_lens, lens):
+    """One call for the first two requests and one for the others, on slices of cu, lens and table: each writes its own
+    requests' rows and no others."""
+    c = attn_case(q_lens, lens, P, 16, hq, hk, D, dtype, pad=3)
+    n = sum(q_lens)
+    out = torch.full_like(c["q"], 7.0)
+    for part in (slice(0, 2), slice(2, None)):
+        cu = c["cu"][part.start:(part.stop + 1) if part.stop else None]
+        before = out.clone()
+        got, lse = kv().prefix_attention(**dict(c, cu=cu, lens=c["lens"][part], table=c["table"][part]), out=out,
+                                         return_lse=True)
+        a, b = int(cu[0]), int(cu[-1])
+        assert torch.equal(out[:a], before[:a]) and torch.equal(out[b:], before[b:])
+        want, wl, to, tl = ref.attention(**dict(c, q=c["q"][:n]))
+        assert bool(((got[a:b].double() - want[a:b]).abs() <= to[a:b]).all())
+        seen = wl[a:b] > -math.inf
+        assert bool((((lse[a:b].double() - wl[a:b]).abs() <= tl[a:b]) | ~seen).all())
