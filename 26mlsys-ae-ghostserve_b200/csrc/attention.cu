@@ -51,6 +51,11 @@ __global__ void __launch_bounds__(kRowThreads) attend_row_kernel(const AttnArgs 
   const int rest = (int)(blockIdx.x - t * (a.hk * parts)), kh = rest / parts, g0 = (rest - kh * parts) * G;
   const int h0 = kh * a.group + g0, nh = a.group - g0 < G ? a.group - g0 : G;
   const int total = a.cu[a.batch] < a.tokens ? a.cu[a.batch] : (int)a.tokens;
+  const int64_t room = (int64_t)a.width * a.page;
+  if (blockIdx.x == 0)  // what is cut below
+    for (int i = threadIdx.x; i < a.batch; i += kRowThreads)
+      if (a.cu[i] < 0 || a.cu[i + 1] < a.cu[i] || a.cu[i + 1] > a.tokens || a.lens[i] < 0 || a.lens[i] > room)
+        atomicOr(&g_attn_status, 1u);
   if (t >= total || t < a.cu[0]) return;  // rows outside the requests stay as they are
   // the request of token t: the last r with cu[r] <= t
   int r = 0, hi = a.batch;
@@ -61,10 +66,9 @@ __global__ void __launch_bounds__(kRowThreads) attend_row_kernel(const AttnArgs 
     else
       hi = mid;
   }
-  const int64_t room = (int64_t)a.width * a.page;
   const int64_t len = a.lens[r] < room ? a.lens[r] : room;
-  if (threadIdx.x == 0 && a.lens[r] > room) atomicOr(&g_attn_status, 1u);
-  const int64_t n = a.cu[r + 1] - a.cu[r], j = t - a.cu[r];
+  const int c0 = a.cu[r] < 0 ? 0 : a.cu[r], c1 = a.cu[r + 1] < total ? a.cu[r + 1] : total;
+  const int64_t n = c1 - c0, j = t - c0;
   int64_t own = len - n + j + 1;
   own = own < 0 ? 0 : (own > len ? len : own);
   const int32_t keys = (int32_t)(a.prefix_len + own);

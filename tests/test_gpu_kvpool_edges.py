@@ -107,3 +107,29 @@ def test_parts_of_a_batch_share_queries_and_out(dtype, hq, hk, D, P, q_lens, len
         assert bool(((got[a:b].double() - want[a:b]).abs() <= to[a:b]).all())
         seen = wl[a:b] > -math.inf
         assert bool((((lse[a:b].double() - wl[a:b]).abs() <= tl[a:b]) | ~seen).all())
+
+
+# ------------------------------------------- lengths that do not fit, flagged ---
+@pytest.mark.parametrize("dtype,hq,hk,D", [(BF, 4, 2, 128), (F4, 4, 2, 64), (BF, 4, 2, 256)])
+@pytest.mark.parametrize("P", [0, 33])
+def test_lengths_that_do_not_fit_are_cut_and_flagged(dtype, hq, hk, D, P):
+    """With and without the tensor core: the same cuts, the same bit."""
+    c = attn_case([1, 4, 2], [40, 20, 30], P, 16, hq, hk, D, dtype, garbage=0.0)
+    status = pkg("codec").device_status
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    room = c["table"].shape[1] * 16
+    c["table"] = torch.where(c["table"] < 0, 0, c["table"])
+    cases = [  # what is given, what is answered
+        (dict(cu=i32([0, 1, 5, 9])), dict(cu=i32([0, 1, 5, 7]))),       # the batch past the queries
+        (dict(cu=i32([0, 1, 9, 9])), dict(cu=i32([0, 1, 7, 7]))),
+        (dict(lens=i32([40, -3, 30])), dict(lens=i32([40, 0, 30]))),    # a negative length
+        (dict(lens=i32([40, 20, room + 1])), dict(lens=i32([40, 20, room]))),
+        (dict(cu=i32([0, 1, 1, 7]), lens=i32([40, room + 9, 30])),      # of a request without queries
+         dict(cu=i32([0, 1, 1, 7]), lens=i32([40, room, 30]))),
+    ]
+    for given, cut in cases:
+        want = kv().prefix_attention(**dict(c, **cut), return_lse=True)
+        assert status() == 0
+        got = kv().prefix_attention(**dict(c, **given), return_lse=True)
+        assert status(clear=True) == 1 << 19
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
