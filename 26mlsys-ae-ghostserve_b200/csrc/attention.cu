@@ -536,7 +536,7 @@ struct TileShared {
   uint64_t piece_full[kPieces], piece_empty[kPieces];
   Piece piece[kPieces];
   Start first;                      // where this CTA's stretch starts
-  int total;
+  int total, wsum[kTileThreads / 32];  // units of the line, of each warp's requests
   uint32_t tmem;
   int quit[2];                      // a wait gave up; after so many turns: more than the CTA's stretch can take
   int bad;                          // a page was outside the pool
@@ -714,7 +714,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
   const int live = live_tokens(a);
   {
     Walk w(a, p, live);
-    int* wsum = reinterpret_cast<int*>(smem);  // the tiles' memory is not in use yet
+    // not in the tiles' memory: tensor copies write that, and nothing would order them behind these words
+    int* wsum = sh.wsum;
     const int per = (a.batch + kTileThreads - 1) / kTileThreads;
     const int r0 = tid * per < a.batch ? tid * per : a.batch, r1 = r0 + per < a.batch ? r0 + per : a.batch;
     int mine = 0, one = 0;  // units of the run, of one head of its last request
