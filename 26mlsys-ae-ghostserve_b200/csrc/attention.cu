@@ -394,7 +394,9 @@ struct Walk {
   // Units of the segment and of the first m (whole) blocks of a head. A block's
   // own keys grow by 256 / group tokens from one to the next; taken as a straight
   // line, the sums have a closed form, and where the line is off the true count
-  // only the balance is.
+  // only the balance is. A segment has fewer than 2^30 units (2^30 keys, blocks of
+  // 2^30 rows), a head and the line more than 32 bits hold: many queries count
+  // as if each block saw 256 / group keys more than the one before, on few keys too.
   __device__ __forceinline__ int base_units() const {
     const int more = g.len - g.ntok;
     return prefix_part() * kUnitTile + (more > 0 ? more / (kKeys / kUnitTile) : 0);
@@ -404,8 +406,8 @@ struct Walk {
     const int u = base_units() + slope() * (g.blk + 1);
     return kUnitSegment + (pair() ? u : u / 2 + (p.run ? 0 : u / 8));
   }
-  __device__ __forceinline__ int units_before(int m) const {
-    return (int)((int64_t)m * (kUnitSegment + base_units()) + (int64_t)m * (m + 1) / 2 * slope());
+  __device__ __forceinline__ int64_t units_before(int m) const {
+    return (int64_t)m * (kUnitSegment + base_units()) + (int64_t)m * (m + 1) / 2 * slope();
   }
   // Tiles of the segment that begin before unit y of it: any rule will do that
   // only grows with y, from 0 to all of them.
@@ -413,17 +415,18 @@ struct Walk {
     const int u = units();
     if (y >= u) return g.tiles;
     if (y <= kUnitSegment) return 0;
-    return (int)__fmul_rn((float)(y - kUnitSegment), __fdiv_rn((float)g.tiles, (float)(u - kUnitSegment)));
+    const int i = (int)__fmul_rn((float)(y - kUnitSegment), __fdiv_rn((float)g.tiles, (float)(u - kUnitSegment)));
+    return i < g.tiles ? i : g.tiles;
   }
   // Units of one head of the row space.
-  __device__ __forceinline__ int head_units() {
+  __device__ __forceinline__ int64_t head_units() {
     if (g.nblk == 0) return 0;
     g.blk = g.nblk - 1;
     return units_before(g.blk) + units();
   }
-  // To the segment that holds unit y of the row space, `one` units a head; y becomes the unit in the segment.
-  __device__ __forceinline__ void seek(int& y, int one) {
-    g.kh = y / one;
+  // To the segment that holds unit y of the row space, `one` units a head; returns the unit in the segment.
+  __device__ __forceinline__ int seek(int64_t y, int64_t one) {
+    g.kh = (int)(y / one);
     y -= g.kh * one;
     int lo = 0, hi = g.nblk;  // the last block that begins at or before y
     while (hi - lo > 1) {
@@ -434,8 +437,8 @@ struct Walk {
         hi = mid;
     }
     g.blk = lo;
-    y -= units_before(lo);
     size();
+    return (int)(y - units_before(lo));
   }
   // The next segment of the line.
   __device__ __forceinline__ void next() {
@@ -455,7 +458,7 @@ struct Walk {
 };
 
 // Units of one head of the prefix's row space.
-__device__ __forceinline__ int prefix_head_units(Walk& w) {
+__device__ __forceinline__ int64_t prefix_head_units(Walk& w) {
   if (w.p.joint || w.a.prefix_len == 0) return 0;
   w.prefix();
   return w.head_units();
@@ -489,8 +492,8 @@ __device__ __forceinline__ int tile_sixteens(const Piece& g, int i) {
   return i == g.tail[0] ? g.tail_keys[0] : (i == g.tail[1] ? g.tail_keys[1] : kKeys / 16);
 }
 
-__device__ __forceinline__ int share(int total, int ctas) {
-  const int n = (total + ctas - 1) / ctas;
+__device__ __forceinline__ int64_t share(int64_t total, int ctas) {
+  const int64_t n = (total + ctas - 1) / ctas;
   return n < kMinShare ? kMinShare : n;
 }
 
@@ -536,7 +539,7 @@ struct TileShared {
   uint64_t piece_full[kPieces], piece_empty[kPieces];
   Piece piece[kPieces];
   Start first;                      // where this CTA's stretch starts
-  int total, wsum[kTileThreads / 32];  // units of the line, of each warp's requests
+  int64_t total, unit, wsum[kTileThreads / 32];  // units of the line, of a stretch, of each warp's requests
   uint32_t tmem;
   int quit[2];                      // a wait gave up; after so many turns: more than the CTA's stretch can take
   int bad;                          // a page was outside the pool
@@ -715,41 +718,41 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
   {
     Walk w(a, p, live);
     // not in the tiles' memory: tensor copies write that, and nothing would order them behind these words
-    int* wsum = sh.wsum;
+    int64_t* wsum = sh.wsum;
     const int per = (a.batch + kTileThreads - 1) / kTileThreads;
     const int r0 = tid * per < a.batch ? tid * per : a.batch, r1 = r0 + per < a.batch ? r0 + per : a.batch;
-    int mine = 0, one = 0;  // units of the run, of one head of its last request
+    int64_t mine = 0, one = 0;  // units of the run, of one head of its last request
     for (int r = r0; r < r1; ++r) {
       w.request(r);
       one = w.head_units();
       mine += one * a.hk;
       if (blockIdx.x == 0 && !w.fits(r)) atomicOr(&g_attn_status, 1u);
     }
-    int x = mine;
+    int64_t x = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, d);
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
       if (lane >= d) x += y;
     }
     if (lane == 31) wsum[warp] = x;
-    const int pre_one = prefix_head_units(w), pre = pre_one * a.hk;
+    const int64_t pre_one = prefix_head_units(w), pre = pre_one * a.hk;
     __syncthreads();
-    int at = pre + x - mine, total = pre;
+    int64_t at = pre + x - mine, total = pre;
 #pragma unroll
     for (int i = 0; i < kTileThreads / 32; ++i) {
-      const int v = wsum[i];
+      const int64_t v = wsum[i];
       if (i < warp) at += v;
       total += v;
     }
-    const int x0 = (int)blockIdx.x * share(total, p.ctas);
+    const int64_t unit = share(total, p.ctas), x0 = blockIdx.x * unit;
     if (tid == 0) {
       sh.total = total;
+      sh.unit = unit;
       // a wait may last as long as a piece; a unit of the line takes 70 ns, a turn 20 and more
-      sh.quit[1] = (1 << 24) + 64 * (share(total, p.ctas) < 1 << 24 ? share(total, p.ctas) : 1 << 24);
+      sh.quit[1] = (1 << 24) + 64 * (unit < 1 << 24 ? (int)unit : 1 << 24);
       if (x0 < pre) {
         w.prefix();
-        sh.first.y = x0;
-        w.seek(sh.first.y, pre_one);
+        sh.first.y = w.seek(x0, pre_one);
         sh.first.g = w.g;
       }
     }
@@ -760,9 +763,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
       }
       if (x0 >= at && x0 < at + one * a.hk) {
         w.request(r);
-        int y = x0 - at;
-        w.seek(y, one);
-        sh.first.y = y;
+        sh.first.y = w.seek(x0 - at, one);
         sh.first.g = w.g;
       }
       at += one * a.hk;
@@ -774,8 +775,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
     tc::fence_after();
   }
   const uint32_t tmem = sh.tmem;
-  const int unit = share(sh.total, p.ctas);
-  const int x0 = (int)blockIdx.x * unit, x1 = sh.total - x0 < unit ? sh.total : x0 + unit;
+  const int64_t unit = sh.unit, x0 = blockIdx.x * unit, x1 = sh.total - x0 < unit ? sh.total : x0 + unit;
   volatile int* quit = sh.quit;
   const float c = fabsf(a.scale) * 1.4426950408889634f;
   if (x0 < x1 && !*quit) {
@@ -1119,14 +1119,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
       constexpr uint32_t kPanel = kRows * 128;
       Walk w(a, p, live);
       w.g = sh.first.g;
-      int y = sh.first.y, left = x1 - x0, at = x0 - y;          // units into the segment, left of the stretch; its start
+      int y = sh.first.y;                                       // units into the segment
+      int64_t left = x1 - x0, at = x0 - y;                      // left of the stretch; the segment's start
       uint32_t n_q = 0, pi = 0;
       bool ok = true;
 #pragma unroll 1
       while (true) {
         const int units = left > 0 ? w.units() : 0;
         const int off = left > 0 && y > 0 ? w.tile_at(y) : 0;
-        const int end = left <= 0 ? 0 : (left >= units - y ? w.g.tiles : w.tile_at(y + left));
+        const int end = left <= 0 ? 0 : (left >= units - y ? w.g.tiles : w.tile_at(y + (int)left));
         if (left > 0 && end == off) {                           // no tile of the segment begins here
           left -= units - y;
           at += units;
@@ -1158,8 +1159,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
             g.len = w.g.len;
             g.kind = (whole && p.joint ? 1 : 0) | (end == w.g.tiles ? 2 : 0) | (whole ? 4 : 0);
             if (!whole) {
-              int c0 = at / unit;                               // the stretch in which its first tile begins
-              while (c0 < (int)blockIdx.x && w.tile_at((c0 + 1) * unit - at) == 0) ++c0;
+              int c0 = (int)(at / unit);                        // the stretch in which its first tile begins
+              const auto before = [&](int64_t v) { return w.tile_at(v < INT_MAX ? (int)v : INT_MAX); };
+              while (c0 < (int)blockIdx.x && before((c0 + 1) * unit - at) == 0) ++c0;
               g.c0 = c0;
             }
           }
@@ -1450,13 +1452,8 @@ int launch_tiles(const AttnArgs& a, cudaStream_t s) {
   p.q_ratio = p.q_run < 4 && a.q_pitch % a.q_head == 0 && a.tokens * (a.q_pitch / a.q_head) < INT_MAX
                   ? (int)(a.q_pitch / a.q_head)
                   : 0;
-  // the line is counted in 32 bits
-  const int64_t keys = (int64_t)a.prefix_len + (int64_t)a.width * a.page;
-  const int64_t blocks = a.tokens * a.group / kBlock + a.batch + 1;  // of the requests, and of the prefix
-  GSEC_REQUIRE((double)blocks * 2 * a.hk * ((keys / kKeys + 3.0) * kUnitTile + kUnitSegment) < 2.0e9 &&
-                   a.tokens * a.group < (1ll << 30),
-               "prefix_attention: %lld tokens on %lld keys are too many for one call", (long long)a.tokens,
-               (long long)keys);
+  GSEC_REQUIRE(a.tokens * a.group < (1ll << 30), "prefix_attention: %lld tokens of %d heads on a KV head are too many",
+               (long long)a.tokens, a.group);
   PoolMaps maps;
   bool ok = true;
   for (int kv = 0; kv < 2; ++kv) {

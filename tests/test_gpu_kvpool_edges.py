@@ -133,3 +133,66 @@ def test_lengths_that_do_not_fit_are_cut_and_flagged(dtype, hq, hk, D, P):
         got = kv().prefix_attention(**dict(c, **given), return_lse=True)
         assert status(clear=True) == 1 << 19
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# ----------------------------------------------------- lengths of the work -----
+@pytest.mark.parametrize("T,hq,hk", [(400_000, 32, 8), (20_000, 1024, 1), (700_000, 4, 4)])
+@pytest.mark.parametrize("P", [0, 3])
+def test_many_queries_on_few_keys(T, hq, hk, P):
+    """All but the last 16 tokens see nothing, or the prefix alone."""
+    c = attn_case([16], [16], P, 16, hq, hk, 16, BF, garbage=0.0)
+    few = c["q"]
+    c["q"] = torch.zeros(T, hq, 16, device="cuda", dtype=BF)
+    c["q"][-16:] = few
+    c["q"][:5] = few[:5]
+    c["cu"] = torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    o, lse = kv().prefix_attention(**c, out=torch.full_like(c["q"], 7.0), return_lse=True)
+    want = attn_case([16], [16], P, 16, hq, hk, 16, BF, garbage=0.0)
+    check_rows(o[-16:], lse[-16:], want, torch.ones(16, hq, dtype=torch.bool, device="cuda"))
+    # zero queries weigh the prefix's values alike
+    first = dict(want, lens=want["lens"] * 0, cu=torch.tensor([0, 5], dtype=torch.int32, device="cuda"), q=few[:5])
+    check_rows(o[:5], lse[:5], first, torch.ones(5, hq, dtype=torch.bool, device="cuda"))
+    rest, ls = o[5:-16], lse[5:-16]
+    assert bool((rest == rest[:1]).all()) and bool((ls == ls[:1]).all())
+    if P == 0:
+        assert bool((rest[0] == 0).all()) and bool((ls[0] == -math.inf).all())
+    else:  # rounding of P and of the result, and of lse: log2, a product
+        slots = (c["prefix"].long()[:, None] * 16 + torch.arange(16, device="cuda")).reshape(-1)[:P]
+        mean = c["pool"][slots, 1].double().mean(0).repeat_interleave(hq // hk, 0)
+        big = c["pool"][slots, 1].double().abs().mean(0).repeat_interleave(hq // hk, 0)
+        assert bool(((rest[0].double() - mean).abs() <= 2 * ref.half_step(BF) * big).all())
+        assert bool(((ls[0].double() - math.log(P)).abs() <= 8 * 2.0 ** -24 * math.log(P)).all())
+
+
+@pytest.mark.parametrize("B,hk,tokens,page", [(2048, 8, 262144, 64), (16384, 8, 32768, 16), (300, 8, 1 << 29, 1 << 17)])
+def test_short_lengths_in_wide_tables(B, hk, tokens, page):
+    """What a table could hold is no work: many requests with tables for long contexts are served, with the same bits
+    as from narrow tables."""
+    g = torch.Generator(device="cuda").manual_seed(B)
+    small = min(page, 64)
+    pool = torch.randn(128 * small, 2, hk, 16, generator=g, device="cuda").to(BF)
+    lens = torch.randint(1, 40, (B,), generator=g, device="cuda", dtype=torch.int32)
+    cu = torch.arange(B + 1, device="cuda", dtype=torch.int32)
+    q = torch.randn(B, hk, 16, generator=g, device="cuda").to(BF)
+    width = tokens // page
+    first = torch.randint(0, 128 * small // page if page <= 64 else 1, (B, 1), generator=g, device="cuda").int()
+    wide = torch.full((B, width), -1, dtype=torch.int32, device="cuda")
+    need = -(-40 // page)
+    wide[:, :need] = (first + torch.arange(need, device="cuda", dtype=torch.int32)) % max(1, 128 * small // page)
+    got = kv().prefix_attention(q, pool, cu, lens, wide, page, return_lse=True)
+    want = kv().prefix_attention(q, pool, cu, lens, wide[:, :need].contiguous(), page, return_lse=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    check_rows(got[0][:50], got[1][:50],
+               dict(q=q[:50], pool=pool, cu=cu[:51], lens=lens[:50], table=wide[:50, :need], page=page, prefix=None,
+                    prefix_len=0), torch.ones(50, hk, dtype=torch.bool, device="cuda"))
+
+
+@pytest.mark.parametrize("q_lens,pad", [([512] + [1] * 15, 0), ([40] + [1] * 15, 0), ([1] * 15 + [40], 1500),
+                                        ([1] * 8 + [300] + [1] * 8, 3)])
+def test_a_chunk_among_decodes(q_lens, pad):
+    """Stacked over the prefix, or each request by itself, as the query count (padding included) has it."""
+    lens = [n + 37 * i for i, n in enumerate(q_lens)]
+    c = attn_case(q_lens, lens, 700, 16, 8, 2, 128, BF, pad=pad)
+    n = sum(q_lens)
+    o, lse = kv().prefix_attention(**c, return_lse=True)
+    check_rows(o[:n], lse[:n], dict(c, q=c["q"][:n]), torch.ones(n, 8, dtype=torch.bool, device="cuda"))

@@ -104,3 +104,8 @@ def test_wrappers_need_cuda_tensors():
         k.qk_norm_rope_store(torch.zeros(4, 64), None, i, i, None, None, 2)
     with pytest.raises(ValueError, match="q must be a CUDA tensor"):
         k.prefix_attention(q=torch.zeros(4, 2, 64), pool=None, cu=i, lens=i, table=i[None], page=16)
+
+
+def test_prefix_attention_refuses_more_rows_than_it_counts():
+    with pytest.raises(ValueError, match="too many"):
+        pkg("_lib").call("gsec_prefix_attention", *attn_args(tokens=1 << 27, hq=8, hk=1, slot_pitch=512, plane=256))
