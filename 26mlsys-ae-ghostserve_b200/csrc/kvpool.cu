@@ -57,6 +57,12 @@ __global__ void __launch_bounds__(kPlanThreads) slots_plan_kernel(const SlotPlan
     bad |= o < 0 || n < 0;
     o = o < 0 ? 0 : o;
     n = n < 0 ? 0 : n;
+    // a length or a position past 32 bits does not exist
+    const int32_t top = (a.base > 0 ? INT_MAX - a.base : INT_MAX) - o;
+    if (n > 0 && n > top) {
+      n = top < 0 ? 0 : top;
+      bad = true;
+    }
     const uint32_t have = a.page_div.div((uint32_t)o + a.page - 1);
     uint32_t want = a.page_div.div((uint32_t)o + (uint32_t)n + a.page - 1);
     bad |= want > (uint32_t)a.width;

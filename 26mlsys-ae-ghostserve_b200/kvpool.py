@@ -73,8 +73,9 @@ def slots_plan(lens: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free:
     ``tokens`` is the size of the per-token outputs (at least ``new.sum()``; a
     batch padded for a captured graph has more), ``base`` is added to every
     position (the length of a shared prefix). Too few free pages, a row longer
-    than the table, more tokens than ``tokens`` or a negative length give slot -1
-    where a token has no place, and set bit 17 of ``codec.device_status``."""
+    than the table, more tokens than ``tokens``, a negative length or one that passes
+    2^31 - 1 (cut to it, ``base`` included) give slot -1 where a token has no place,
+    and set bit 17 of ``codec.device_status``."""
     if stream is not None:
         with _on(stream, lens):
             return slots_plan(lens, new, table, free, cursor, page, tokens, base)

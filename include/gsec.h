@@ -174,7 +174,8 @@ enum { GSEC_BF16 = 0, GSEC_F16 = 1, GSEC_F32 = 2 };
  * from cu[batch] to capacity get slot -1 and position 0. All arrays are on the
  * device; slots and positions are 16-byte aligned; lens_out and cursor_out are
  * not lens and cursor. Missing free pages, a row past `width`, tokens past
- * `capacity` or a negative length set bit 17 of gsec_device_status; a token
+ * `capacity`, a negative length or one that takes lens_out or a position past
+ * 2^31 - 1 (cut to it) set bit 17 of gsec_device_status; a token
  * without a page gets slot -1. */
 GSEC_API int gsec_slots_plan(const int32_t* lens, const int32_t* new_lens, int32_t batch, int32_t* table,
                     int64_t table_pitch, int32_t width, const int32_t* free_pages, int64_t nfree,

@@ -196,3 +196,27 @@ def test_a_chunk_among_decodes(q_lens, pad):
     n = sum(q_lens)
     o, lse = kv().prefix_attention(**c, return_lse=True)
     check_rows(o[:n], lse[:n], dict(c, q=c["q"][:n]), torch.ones(n, 8, dtype=torch.bool, device="cuda"))
+
+
+def test_slots_plan_of_lengths_at_the_end_of_32_bits():
+    status, top = pkg("codec").device_status, 2 ** 31 - 1
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+
+    def plan(lens, new, page, tokens, base=0, width=2):
+        table = i32([[3, 5, 1, 2][:width]] * len(lens))
+        p = kv().slots_plan(i32(lens), i32(new), table, i32([7, 8, 9]), i32([0]), page, tokens, base=base)
+        assert table.tolist() == [[3, 5, 1, 2][:width]] * len(lens)
+        return [x.tolist() for x in (p.slots, p.positions, p.cu, p.lens, p.cursor)]
+
+    # the last length that exists
+    assert plan([top - 1], [1], 1 << 30, 1) == [[5 * 2 ** 30 + 2 ** 30 - 2], [top - 1], [0, 1], [top], [0]]
+    assert plan([top - 6], [1], 1 << 30, 1, base=5) == [[5 * 2 ** 30 + 2 ** 30 - 7], [top - 1], [0, 1], [top - 5], [0]]
+    assert plan([top], [0], 1 << 30, 1) == [[-1], [0], [0, 0], [top], [0]]
+    assert status() == 0
+    # past it: cut and flagged
+    assert plan([top], [1], 1 << 30, 1) == [[-1], [0], [0, 0], [top], [0]]
+    assert status() == 1 << 17
+    assert plan([top - 4], [3], 1 << 30, 3, base=3) == [[5 * 2 ** 30 + 2 ** 30 - 5, -1, -1], [top - 1, 0, 0], [0, 1], [top - 3], [0]]
+    assert status() == 1 << 17
+    assert plan([top, 1], [top, 1], 16, 1, width=4) == [[3 * 16 + 1], [1], [0, 0, 1], [top, 2], [0]]
+    assert status() == 1 << 17
