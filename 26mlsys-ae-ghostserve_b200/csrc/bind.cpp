@@ -13,10 +13,12 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
 #include <cstdarg>
+#include <exception>
 #include <string>
 
 #include "gsec.h"
@@ -181,8 +183,8 @@ PyObject* guarded(F f) {
   try {
     return f();
   } catch (const Refused&) {
-  } catch (const std::exception& e) {  // an allocation that failed, and the like
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {  // an allocation that failed (torch.OutOfMemoryError), and the like
+    torch::translate_exception_to_python(std::current_exception());
   }
   return nullptr;
 }

@@ -220,3 +220,17 @@ def test_slots_plan_of_lengths_at_the_end_of_32_bits():
     assert status() == 1 << 17
     assert plan([top, 1], [top, 1], 16, 1, width=4) == [[3 * 16 + 1], [1], [0, 0, 1], [top, 2], [0]]
     assert status() == 1 << 17
+
+
+# ------------------------------------------------------ errors of the calls -----
+def test_an_allocation_that_fails_is_an_out_of_memory_error():
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    args = (i32([0]), i32([1]), i32([[-1]]), i32([0]), i32([0]), 16)
+    torch.cuda.empty_cache()
+    torch.cuda.set_per_process_memory_fraction(0.05)  # of 180 GB: below the 12 bytes of each of 2^30 tokens
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            kv().slots_plan(*args, 1 << 30)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert kv().slots_plan(*args, 1).slots.tolist() == [0]
