@@ -71,6 +71,7 @@ double real(PyObject* o) {
 
 void no_grad(const at::Tensor& t, const char* what) {
   NEED(!(t.requires_grad() && c10::GradMode::is_enabled()), "%s requires a gradient: the operator has no backward pass", what);
+  NEED(!t._fw_grad(0).defined(), "%s carries a forward-mode tangent: the operator has no derivative", what);
 }
 
 // The first tensor names the device.
@@ -270,6 +271,8 @@ PyObject* qk_norm_rope_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     auto* cos_at = static_cast<float*>(c.flat(cos, "cos", at::kFloat));
     auto* sin_at = static_cast<float*>(c.flat(sin, "sin", at::kFloat));
+    no_grad(cos, "cos");
+    no_grad(sin, "sin");
     NEED(cos.dim() == 2 && cos.size(1) < (1 << 20), "cos must have shape [positions, rot / 2]");
     NEED(sin.sizes() == cos.sizes(), "sin must have the shape of cos");
     const void* w[2] = {nullptr, nullptr};

@@ -234,3 +234,30 @@ def test_an_allocation_that_fails_is_an_out_of_memory_error():
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
     assert kv().slots_plan(*args, 1).slots.tolist() == [0]
+
+
+def test_forward_mode_tangents_and_angle_gradients_are_refused():
+    """The operators have neither a forward nor a backward derivative: none is dropped in silence."""
+    import torch.autograd.forward_ad as fwd
+    from test_gpu_kvpool import store_case
+    c = attn_case([1, 2], [20, 30], 16, 16, 4, 2, 64, BF)
+    qkv, pool, slots, positions, cos, sin, w = store_case(9, 4, 2, 64, 64, BF, True)
+    base = dict(qkv=qkv, pool=pool, slots=slots, positions=positions, cos=cos, sin=sin, heads=4, q_weight=w[0],
+                k_weight=w[1])
+    for name in ("cos", "sin"):
+        with pytest.raises(ValueError, match="gradient"):
+            kv().qk_norm_rope_store(**dict(base, **{name: base[name].clone().requires_grad_()}))
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for name in ("q", "pool"):
+            with pytest.raises(ValueError, match="tangent"):
+                kv().prefix_attention(**dict(c, **{name: dual(c[name])}))
+        with pytest.raises(ValueError, match="tangent"):
+            kv().prefix_attention(**c, out=dual(torch.zeros_like(c["q"])))
+        for name in ("qkv", "pool", "cos", "sin", "q_weight", "k_weight"):
+            with pytest.raises(ValueError, match="tangent"):
+                kv().qk_norm_rope_store(**dict(base, **{name: dual(base[name])}))
+        with torch.no_grad(), pytest.raises(ValueError, match="tangent"):  # forward derivatives stay on there
+            kv().prefix_attention(**dict(c, q=dual(c["q"])))
+        kv().prefix_attention(**c)
+        kv().qk_norm_rope_store(**base)
