@@ -14,9 +14,11 @@ from __future__ import annotations
 
 import concurrent.futures as cf
 import glob
+import importlib.metadata
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -33,12 +35,23 @@ CFLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-fvisibility=hi
 
 BIND = os.path.join(CSRC, "bind.cpp")
 BIND_LIB = os.path.join(LIBDIR, "gsec_torch.so")
+BIND_STAMP = os.path.join(BUILD, "gsec_torch.built_with")  # the torch and Python that BIND_LIB was built with
+
+
+def _bind_versions() -> str:
+    return f"torch {importlib.metadata.version('torch')}, {sysconfig.get_config_var('SOABI')}"
+
+
+def _bind_stale() -> bool:
+    """Whether BIND_LIB is missing, older than its sources, or built with another torch or Python."""
+    if _stale(BIND_LIB, [BIND, *_headers()]) or not os.path.exists(BIND_STAMP):
+        return True
+    with open(BIND_STAMP) as f:
+        return f.read() != _bind_versions()
 
 
 def _build_bind(verbose: bool) -> None:
     """lib/gsec_torch.so: a Python module on top of libgsec.so (found beside it at run time)."""
-    import sysconfig
-
     import torch
     from torch.utils import cpp_extension
 
@@ -54,6 +67,8 @@ def _build_bind(verbose: bool) -> None:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for {BIND}:\n{r.stdout}\n{r.stderr}")
+    with open(BIND_STAMP, "w") as f:
+        f.write(_bind_versions())
 
 
 def _headers():
@@ -106,7 +121,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_v: bool = False) -> 
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
-    if force or _stale(BIND_LIB, [BIND, *hdrs]):
+    if force or _bind_stale():
         _build_bind(verbose)
     return LIB
 
