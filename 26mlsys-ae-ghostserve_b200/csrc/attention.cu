@@ -1106,10 +1106,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
         }
         done_piece(pi);
       }
-      // copies must not outlive the CTA: all are waited for by the products, unless a wait gave up
-      if (*quit)
-        for (uint32_t q = pos > turns ? pos - turns : 0; q < pos; ++q)
-          (void)pipe::bar_wait(sh.full + stage0 + q % turns, (q / turns) & 1);
+      // copies must not outlive the CTA, and whoever waits for the last of them may still give up
+      for (uint32_t q = pos > turns ? pos - turns : 0; q < pos; ++q)
+        (void)pipe::bar_wait(sh.full + stage0 + q % turns, (q / turns) & 1);
     } else {
       // ------------------------------------------ the walk, loads of Q ----
       // Row x of a block is head x % group of token x / group: boxes of whole groups
@@ -1215,23 +1214,24 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tile_kernel(const Attn
         y = 0;
         if (left > 0) w.next();
       }
-      if (*quit)
-        for (uint32_t q = n_q > 2 ? n_q - 2 : 0; q < n_q; ++q) (void)pipe::bar_wait(sh.q_full + (q & 1), (q >> 1) & 1);
+      for (uint32_t q = n_q > 2 ? n_q - 2 : 0; q < n_q; ++q) (void)pipe::bar_wait(sh.q_full + (q & 1), (q >> 1) & 1);
     }
     }
-  }
-  // No product may be in flight when tensor memory is given back: the softmax
-  // warps have waited for the last of them, unless a wait gave up.
-  if (warp == 8 && *quit) {
-    const uint64_t t0 = pipe::now_ns();
-    while (pipe::now_ns() - t0 < 1000000ull) {
-    }
-    __syncwarp();
   }
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  if (warp == 8) tc::dealloc(tmem, 512);
+  // No product may be in flight when tensor memory is given back: the softmax
+  // warps have waited for the last of them, unless a wait gave up.
+  if (warp == 8) {
+    if (*quit) {
+      const uint64_t t0 = pipe::now_ns();
+      while (pipe::now_ns() - t0 < 1000000ull) {
+      }
+      __syncwarp();
+    }
+    tc::dealloc(tmem, 512);
+  }
   if (tid == 0 && (sh.quit[0] || sh.bad)) atomicOr(&g_attn_status, (sh.quit[0] ? 2u : 0u) | (sh.bad ? 1u : 0u));
 }
 
