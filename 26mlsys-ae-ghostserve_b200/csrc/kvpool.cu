@@ -218,17 +218,28 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
+// 16 bytes that are read once. Like every load of this file it stays behind
+// grid_dep_wait(): the kernel before may still be writing them.
+__device__ __forceinline__ uint4 load_once(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+
 // Four values of a cos or sin row (two for 32-bit pairs of neighbours).
 template <int N>
 __device__ __forceinline__ void load_angles(const float* at, float* f) {
   if (N == 2) {
-    const float2 v = __ldg(reinterpret_cast<const float2*>(at));
+    const float2 v = *reinterpret_cast<const float2*>(at);
     f[0] = v.x;
     f[1] = v.y;
   } else {
 #pragma unroll
     for (int e = 0; e < N; e += 4) {
-      const float4 v = __ldg(reinterpret_cast<const float4*>(at + e));
+      const float4 v = *reinterpret_cast<const float4*>(at + e);
       f[e] = v.x;
       f[e + 1] = v.y;
       f[e + 2] = v.z;
@@ -238,7 +249,7 @@ __device__ __forceinline__ void load_angles(const float* at, float* f) {
 }
 
 __device__ __forceinline__ int64_t index_at(const void* p, int bytes, uint32_t i) {
-  return bytes == 8 ? __ldg(static_cast<const long long*>(p) + i) : (int64_t)__ldg(static_cast<const int*>(p) + i);
+  return bytes == 8 ? static_cast<const int64_t*>(p)[i] : (int64_t)static_cast<const int32_t*>(p)[i];
 }
 
 // G and the kind of pairs are compile-time: the shuffles of a loop whose length is
@@ -263,7 +274,7 @@ __global__ void __launch_bounds__(kStoreThreads) qk_store_kernel(const QkStoreAr
   uint4 raw[H];
 #pragma unroll
   for (int j = 0; j < H; ++j)
-    raw[j] = live && j < nh ? __ldcs(reinterpret_cast<const uint4*>(row + j * a.dim * (int)sizeof(T))) : vzero();
+    raw[j] = live && j < nh ? load_once(row + j * a.dim * (int)sizeof(T)) : vzero();
   int64_t slot = -1;
   if (kind && nh > 0) {
     slot = index_at(a.slots, a.slot_bytes, t);
@@ -314,8 +325,8 @@ __global__ void __launch_bounds__(kStoreThreads) qk_store_kernel(const QkStoreAr
     }
     if (w != nullptr && live) {
       float wf[N], wp[N];
-      V::unpack(__ldg(reinterpret_cast<const uint4*>(w) + lane), wf);
-      V::unpack(__ldg(reinterpret_cast<const uint4*>(w) + partner), wp);
+      V::unpack(reinterpret_cast<const uint4*>(w)[lane], wf);
+      V::unpack(reinterpret_cast<const uint4*>(w)[partner], wp);
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         c[e] *= wf[e];

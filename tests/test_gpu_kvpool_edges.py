@@ -261,3 +261,18 @@ def test_forward_mode_tangents_and_angle_gradients_are_refused():
             kv().prefix_attention(**dict(c, q=dual(c["q"])))
         kv().prefix_attention(**c)
         kv().qk_norm_rope_store(**base)
+
+
+@pytest.mark.parametrize("dtype,hq,hk,D", [(F4, 4, 2, 64), (BF, 4, 2, 256)])
+def test_pages_outside_the_pool_without_the_tensor_core(dtype, hq, hk, D):
+    """They read as zeros and are flagged."""
+    c = attn_case([1, 1], [40, 20], 32, 16, hq, hk, D, dtype)
+    zero = c["pool"].clone()
+    zero[c["table"][0, 1].item() * 16:][:16] = 0
+    zero[c["prefix"][1].item() * 16:][:16] = 0
+    want = kv().prefix_attention(**dict(c, pool=zero), return_lse=True)
+    table, prefix = c["table"].clone(), c["prefix"].clone()
+    table[0, 1], prefix[1] = -1, c["pool"].shape[0] // 16
+    got = kv().prefix_attention(**dict(c, table=table, prefix=prefix), return_lse=True)
+    assert pkg("codec").device_status(clear=True) == 1 << 19
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
