@@ -447,3 +447,55 @@ def hook_pool_chunk(rank, world, port, backend, out):
     dist.all_gather_object(oks, ok)
     out.put((rank, all(oks), [r["chunk_id"] for r in ft.records]))
     dist.destroy_process_group()
+
+
+def hook_plan(rank, world, port, backend, out):
+    """A serving step's own slot list through the hook: a padded slot plan, the store of
+    its tokens, protection by the patched extend call with the plan's slots (the
+    padding's -1 among them), loss of rank 1's new rows, recover_pool through the
+    same slots, and attention over the rebuilt pool: the bits of before."""
+    _init(rank, world, port, backend)
+    torch.cuda.set_device(rank if backend == "nccl" else 0)
+    hook, kv = _pkg("hook"), _pkg("kvpool")
+    from types import SimpleNamespace
+
+    class FlashInferAttnBackend:
+        kv_buffer = torch.randn(256, 2, 2, 64, device="cuda",
+                                generator=torch.Generator(device="cuda").manual_seed(rank)).to(torch.bfloat16)
+
+        def forward_extend(self, batch, layer=None, save_kv_cache=True):
+            return None
+
+    be = FlashInferAttnBackend()
+    ft = hook.KVFaultTolerance(hook.HookConfig(mode="fused", scheme="rdp", unit=256, metrics_file=None))
+    hook.patch_backend(be, ft)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    table = torch.full((3, 4), -1, dtype=torch.int32, device="cuda")
+    lens, cursor, plans, outs = i32([0, 0, 0]), i32([0]), [], []
+    ang = torch.outer(torch.arange(64, device="cuda").float(), 1e4 ** (-torch.arange(32, device="cuda") / 32.0))
+    for step, new in enumerate(([5, 20, 1], [1, 1, 1], [1, 0, 1])):
+        plan = kv.slots_plan(lens, i32(new), table, torch.arange(16, dtype=torch.int32, device="cuda"), cursor, 16, 32)
+        qkv = torch.randn(32, 8 * 64, device="cuda", generator=torch.Generator(device="cuda").manual_seed(step)).to(
+            torch.bfloat16)
+        q = kv.qk_norm_rope_store(qkv, be.kv_buffer, plan.slots, plan.positions, ang.cos(), ang.sin(), 4)
+        be.forward_extend(SimpleNamespace(slot_mapping=plan.slots), layer=0)
+        args = (q[:sum(new)], plan.cu, plan.lens, plan.table.clone())
+        plans.append(plan)
+        outs.append((args, kv.prefix_attention(q[:sum(new)], be.kv_buffer, *args[1:], 16)))
+        lens, cursor = plan.lens, plan.cursor
+    ft.flush()
+    saved = be.kv_buffer.clone()
+    if rank == 1:
+        for plan in plans:
+            be.kv_buffer[plan.slots[plan.slots >= 0]] = 0
+    for cid, plan in enumerate(plans, start=1):
+        ft.recover_pool(cid, [1], be.kv_buffer, plan.slots)
+    args, want = outs[-1]
+    ok = torch.equal(be.kv_buffer, saved) and torch.equal(
+        kv.prefix_attention(args[0], be.kv_buffer, *args[1:], 16), want)
+    ok = ok and _pkg("codec").device_status() == 0
+    ft.close()
+    oks = [None] * world
+    dist.all_gather_object(oks, ok)
+    out.put((rank, all(oks)))
+    dist.destroy_process_group()
