@@ -59,9 +59,8 @@ __device__ __forceinline__ int64_t key_slot(const AttnArgs& a, int r, int32_t x)
 //   m = max m_g, l = sum l_g 2^(m_g - m), o = sum o_g 2^(m_g - m) / l.
 // Bound by the latency of a step (lookup, loads, sum over the lanes), of which each
 // has several keys: 16 requests of 32 fp32 heads on 8 KV heads of 128, behind 4096
-// keys, 367 us; 256-wide bf16 heads 329. (One head per CTA and a key a step: 715 and
-// 825; G = 2: 400 and 337.) Not split over long keys: few rows behind a long
-// cache leave SMs idle.
+// keys, 283 us; 256-wide bf16 heads 319. (G = 1: 418 and 508; G = 2: 392 and 326.)
+// Not split over long keys: few rows behind a long cache leave SMs idle.
 constexpr int kRowThreads = 256;
 
 template <typename T, int NC, int G>
@@ -240,7 +239,9 @@ int launch_rows(const AttnArgs& a, int L, cudaStream_t s) {
                    "prefix_attention");
 }
 
-// Heads together as long as half of the SMs are busy.
+// Heads together as long as half of the SMs are busy. (fp32, groups of 4 on one KV head of
+// 128, 1000 keys, four heads together and one by one: 1 request 65 and 41 us, 8 of them 66
+// and 55; 64 of them 191 and 324.)
 template <typename T, int NC>
 int launch_rows(const AttnArgs& a, int L, cudaStream_t s) {
   const int64_t heads = a.tokens * a.hk;
@@ -285,8 +286,8 @@ int attend_rows(const AttnArgs& a, cudaStream_t s) {
 // memory, and loops are unrolled only as far as they have to be (with the walk in
 // every role and 128-column bodies a one-tile segment took 12000 cycles).
 // Measured (bf16, 32 heads on 8 KV heads of 128, pages of 16): 16 decode requests
-// behind 32768 keys 43 us, 3.7 TB/s; 128 ragged ones behind 2047 150 us, 4.4 TB/s;
-// 256 behind 24576 180 us, 576 TFLOP/s; a 2048-token chunk behind 30720 1140 us, 940
+// behind 32768 keys 42 us, 3.7 TB/s; 128 ragged ones behind 2047 146 us, 4.5 TB/s;
+// 256 behind 24576 182 us, 568 TFLOP/s; a 2048-token chunk behind 30720 1100 us, 970
 // TFLOP/s, power capped (990 us alone). The first two are bound by DRAM and the
 // beginnings and ends of segments, the others by a step's chain: scores, softmax
 // (1700 cycles), sums, and only then the next scores, in the same tensor memory.
@@ -324,6 +325,8 @@ struct Start {           // a point on the line
 };
 
 // Rows of a box of queries: a few, since a piece of a single token has `group` of them.
+// (Boxes of 4: 16 extends of 8 tokens behind 4096 keys 38 us instead of 36, a 2048-token
+// chunk 1075 instead of 1035. Boxes of 64: no difference.)
 constexpr int kQueryBox = 16;
 
 struct TilePlan {
@@ -578,7 +581,13 @@ struct TileShared {
 };
 static_assert(sizeof(TileShared) <= kBehind, "shared memory behind the tiles");
 
-// 16 words of P from 32 scores, their sum and their maximum (with `top`). (Two
+// 16 words of P from 32 scores, their sum and their maximum (with `top`). P is
+// rounded to the type of the values, the only one that the tensor core multiplies
+// with them: each by up to half a step (2^-8 of it in bf16, 2^-11 in fp16, and below
+// 2^-14 half of fp16's smallest step), independently. The sum takes them unrounded, in
+// 32 bits, as are scores, maxima, O and partial results. Beside the rounding of the
+// result that leaves o 0.0023 of its norm off in bf16 and 0.00029 in fp16, where the
+// exact o rounded is 0.0017 and 0.00021 off; lse 5e-8. (Two
 // scores to an instruction, fma.f32x2 and add.f32x2, took longer: 1550 cycles a
 // tile instead of 1290.)
 template <typename T>
@@ -1401,13 +1410,22 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttnArgs a, cons
 // The tensor core takes 16-bit values, sixteen at a time; a head of more than
 // 128 of them, of an odd half of sixteen, or of 32-bit values goes row by row.
 // So does a scale next to nothing, under which a masked score would not vanish.
+// (bf16, 32 heads on 8 KV heads of 128, in tiles and row by row: 16 decode requests behind
+// 4096 keys 22 and 157 us, 128 ragged ones behind 2047 129 and 879, 16 extends of 8 tokens
+// 36 and 958. Only a few short rows would be quicker row by row: three requests of up to
+// 300 keys on one KV head 13.5 and 10.3, one of 1000 keys 13.7 and 24.6.)
 bool takes_tiles(const AttnArgs& a, int dtype) {
   return dtype != GSEC_F32 && a.dim <= 128 && a.dim % 16 == 0 && !(fabsf(a.scale) < 1e-20f);
 }
 
 // Stacking the requests' rows over the prefix pays when they would not fill
 // tiles by themselves; with about a tile of rows each (or one request) prefix and
-// own keys are better taken in one go, which leaves little to join.
+// own keys are better taken in one go, which leaves little to join. (16 extends of 8,
+// 16, 32 and 64 tokens, groups of 4, behind 4096 keys: stacked 36, 45, 71 and 198 us, in
+// one go 58, 58, 57 and 89; a 2048-token chunk behind 30720 keys 1240 and 1030; 256 decode
+// requests behind 24576 177 and 3290. The rule goes by the batch's mean, padding included:
+// a chunk of 512 tokens among 15 decode requests behind 30720 keys, which it takes in one
+// go, is 496 us, stacked 469.)
 TilePlan tile_plan(const AttnArgs& a, int64_t* bytes) {
   TilePlan p{};
   p.ctas = sm_count();
@@ -1513,13 +1531,16 @@ int launch_tiles(const AttnArgs& a, cudaStream_t s) {
       launch_pdl(kernel, dim3((unsigned)p.ctas), dim3(kTileThreads), smem, s, a, p, maps),
       "prefix_attention");
   if (rc) return rc;
-  if (p.joint) {  // a warp to a row of a whole block, or a block to a row of a few
+  // A warp to a row of a whole block, or a block to a row of a few. (8 blocks a segment and
+  // 32: one request of 1000 keys 13.7 us and 17.2, 4 extends of 256 tokens 94 and 91.5.)
+  if (p.joint) {
     const unsigned y = a.tokens * a.group < kBlock ? 8 : kBlock / 8;
     return launch_rc(launch_pdl(attend_join_cuts_kernel<T>, dim3((unsigned)p.ctas, y), dim3(256), 0, s, a, p),
                      "prefix_attention join");
   }
   const int64_t rows = a.tokens * a.hq;
-  // few rows: eight warps to a row, since each may have a part from every CTA
+  // few rows: eight warps to a row, since each may have a part from every CTA. (Eight warps and
+  // one: 16 requests behind 32768 keys 42 us and 53, 256 behind 24576 198 and 177.)
   if (rows <= (int64_t)p.ctas * 16)
     return launch_rc(launch_pdl(attend_join_kernel<T, 8>, dim3((unsigned)rows), dim3(256), 0, s, a, p),
                      "prefix_attention join");

@@ -66,7 +66,7 @@ class SlotPlan(NamedTuple):
 
 def slots_plan(lens: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free: torch.Tensor, cursor: torch.Tensor,
                page: int, tokens: int, base: int = 0, *, stream: Optional[torch.cuda.Stream] = None) -> SlotPlan:
-    """Plan the slots of ``new[i]`` more tokens for each request that has ``lens[i]``.
+    """Plan the slots of ``new[i]`` more tokens for each of 1 to 16384 requests, which has ``lens[i]``.
 
     ``table`` [batch, pages] holds the requests' pages and is filled in place with
     the pages the new tokens need, taken in request order from ``free[cursor:]``.
@@ -125,8 +125,14 @@ def prefix_attention(q: torch.Tensor, pool: torch.Tensor, cu: torch.Tensor, lens
     rows before ``cu[0]`` and from ``cu[-1]`` on are left as they were. Keys and
     values inside a request's length must be finite (a non-finite value may spread to
     earlier tokens of the same request); slots outside all lengths may hold anything.
-    A page outside the pool reads as zeros and a
-    length past the table is cut; both set bit 19 of ``codec.device_status``."""
+    A page outside the pool reads as zeros, a length past the table or a batch past
+    ``q`` is cut; both set bit 19 of ``codec.device_status``.
+
+    Scores, sums and accumulators are held in 32 bits and the result is rounded once.
+    On the tensor core (bf16 and fp16 heads of up to 128 values, in sixteens) a key's
+    weight is rounded to ``q``'s type as well before it meets the value; lse is of the
+    unrounded weights. 1 to 16384 requests, fewer than 2^31 query heads in all and 2^30
+    on a KV head, prefix and table together below 2^30 keys."""
     if stream is not None:
         with _on(stream, q):
             return prefix_attention(q, pool, cu, lens, table, page, prefix, prefix_len, scale, out, return_lse)

@@ -163,7 +163,7 @@ GSEC_API int gsec_slots_scatter(void* pool, int64_t pitch, int64_t plane, int32_
 /* Element types of the serving entries. */
 enum { GSEC_BF16 = 0, GSEC_F16 = 1, GSEC_F32 = 2 };
 
-/* Plan the slots of a batch's new tokens. Request i (batch <= 16384) holds
+/* Plan the slots of a batch's new tokens. Request i (batch 1 to 16384) holds
  * lens[i] tokens on the first ceil(lens[i] / page) pages of its row of `table`
  * ([batch, width] int32, table_pitch elements apart) and gets new_lens[i] more.
  * The pages that needs are taken in request order from free_pages[cursor[0]..)
@@ -209,7 +209,11 @@ GSEC_API int gsec_qk_norm_rope_store(const void* qkv, int64_t qkv_pitch, int64_t
  * tokens cu[i]..cu[i+1) of request i (n of them) attend to the prefix_len keys
  * on the pages `prefix` and to the request's own keys (lens[i], on its row of
  * `table`): token j sees own keys 0 .. lens[i] - n + j. hq / hk query heads read
- * each KV head. out ([tokens, hq, dim]) and lse ([tokens, hq], natural log, may
+ * each KV head (tokens * hq below 2^31, tokens * hq / hk below 2^30; batch 1 to
+ * 16384; prefix_len + width * page below 2^30). Scores, sums and accumulators are
+ * held in 32 bits; on the tensor core (16-bit dtype, dim up to 128 in sixteens) a
+ * key's weight is rounded to dtype before it meets the value, lse is of the
+ * unrounded weights. out ([tokens, hq, dim]) and lse ([tokens, hq], natural log, may
  * be null); a row that sees no key is 0 and -inf, rows before cu[0] and from
  * cu[batch] on are not written. q: byte strides q_pitch (token) and q_head (head), at least a head's
  * bytes each (no broadcast). dim: whole 16-byte
@@ -218,8 +222,8 @@ GSEC_API int gsec_qk_norm_rope_store(const void* qkv, int64_t qkv_pitch, int64_t
  * outside all lengths may hold anything. workspace: 16-byte aligned, of
  * gsec_prefix_attention_workspace bytes (0 with the same tokens, heads and dim
  * means none is needed), not shared by calls that may overlap. A page outside the
- * pool reads as zeros, a length past the table or a batch past `tokens` is cut;
- * both set bit 19 of gsec_device_status. A bounded wait that gives up sets bit
+ * pool reads as zeros, a negative length, one past the table or a batch past
+ * `tokens` is cut; all set bit 19 of gsec_device_status. A bounded wait that gives up sets bit
  * 25. */
 GSEC_API int gsec_prefix_attention(const void* q, int64_t q_pitch, int64_t q_head, int64_t tokens, int32_t dtype,
                           int32_t hq, int32_t hk, int32_t dim, const void* pool, int64_t pitch,
