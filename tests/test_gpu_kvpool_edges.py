@@ -276,3 +276,38 @@ def test_pages_outside_the_pool_without_the_tensor_core(dtype, hq, hk, D):
     got = kv().prefix_attention(**dict(c, table=table, prefix=prefix), return_lse=True)
     assert pkg("codec").device_status(clear=True) == 1 << 19
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# ---------------------------------------------------------------- far and long --
+@pytest.mark.parametrize("dtype,hk,D", [(F4, 8, 64), (BF, 8, 256)])
+def test_rows_in_slots_past_32_bits(dtype, hk, D):
+    """Without the tensor core: pages more than 2^32 bytes into the pool."""
+    c = attn_case([1, 20], [70, 40], 300, 16, hk, hk, D, dtype)
+    rows = 4_400_000_000 // (2 * hk * D * c["pool"].element_size()) // 16 * 16
+    far = torch.empty(rows, 2, hk, D, dtype=dtype, device="cuda")
+    shift = rows // 16 - c["pool"].shape[0] // 16
+    far[shift * 16:shift * 16 + c["pool"].shape[0]] = c["pool"]
+    table = torch.where(c["table"] >= 0, c["table"] + shift, -1)
+    a = kv().prefix_attention(**c, return_lse=True)
+    b = kv().prefix_attention(**dict(c, pool=far, table=table, prefix=c["prefix"] + shift), return_lse=True)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_store_in_slots_past_32_bits():
+    from test_gpu_kvpool import store_case
+    qkv, pool, slots, positions, cos, sin, w = store_case(50, 8, 8, 128, 128, BF, True)
+    rows = 1_100_000  # 4096 bytes each
+    far = torch.zeros(rows, 2, 8, 128, dtype=BF, device="cuda")
+    shift = rows - pool.shape[0]
+    q = kv().qk_norm_rope_store(qkv, pool, slots, positions, cos, sin, 8, q_weight=w[0], k_weight=w[1])
+    f = kv().qk_norm_rope_store(qkv, far, slots + shift, positions, cos, sin, 8, q_weight=w[0], k_weight=w[1])
+    assert torch.equal(q, f) and torch.equal(far[slots + shift], pool[slots])
+    far[slots + shift] = 0
+    assert not bool(far.any())
+
+
+@pytest.mark.parametrize("P,own", [(0, 1_000_003), (600_001, 400_000)])
+def test_a_million_keys(P, own):
+    c = attn_case([2], [own], P, 16, 4, 1, 64, BF)
+    o, lse = kv().prefix_attention(**c, return_lse=True)
+    check_rows(o, lse, c, torch.ones(2, 4, dtype=torch.bool, device="cuda"))
