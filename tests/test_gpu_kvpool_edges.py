@@ -216,7 +216,8 @@ def test_slots_plan_of_lengths_at_the_end_of_32_bits():
     # past it: cut and flagged
     assert plan([top], [1], 1 << 30, 1) == [[-1], [0], [0, 0], [top], [0]]
     assert status() == 1 << 17
-    assert plan([top - 4], [3], 1 << 30, 3, base=3) == [[5 * 2 ** 30 + 2 ** 30 - 5, -1, -1], [top - 1, 0, 0], [0, 1], [top - 3], [0]]
+    assert plan([top - 4], [3], 1 << 30, 3, base=3) == [[5 * 2 ** 30 + 2 ** 30 - 5, -1, -1], [top - 1, 0, 0], [0, 1],
+                                                        [top - 3], [0]]
     assert status() == 1 << 17
     assert plan([top, 1], [top, 1], 16, 1, width=4) == [[3 * 16 + 1], [1], [0, 0, 1], [top, 2], [0]]
     assert status() == 1 << 17
